@@ -23,6 +23,10 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 OBJ_DIR = os.path.join(REPO_DIR, "build", "obj")
 ARCH = os.environ.get("PCA_OFFLOAD_ARCH", "gfx950")
 EXT_NAME = "_C"
+# Device code without packed fp32 instructions: -O3 forms v_pk_add/mul/fma_f32 from plain float code
+# by itself, and some of their forms have given wrong results on MI355X. (The host pass warns that
+# it does not know the feature; the warning means nothing.)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def ext_path() -> str:
@@ -124,7 +128,7 @@ def _needs_build(src: str, obj: str, deps) -> bool:
 def _compile(src, obj, flags, verbose):
     cmd = [_hipcc()] + flags
     if src.endswith(".hip"):
-        cmd += ["-x", "hip", f"--offload-arch={ARCH}"]
+        cmd += ["-x", "hip", f"--offload-arch={ARCH}", *NO_PACKED_FP32]
     cmd += ["-c", src, "-o", obj]
     if verbose:
         print(" ".join(cmd), flush=True)
