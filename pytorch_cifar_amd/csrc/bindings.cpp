@@ -242,6 +242,8 @@ void direct_wgrad_launch(const bf16*, const bf16*, int, int, int, int, int, int,
                          int, int, int, int, float*, int, float*, hipStream_t);
 // comm.cpp
 void register_comm(py::module& m);
+// bindings_distill.cpp
+void register_distill(py::module& m);
 void set_deterministic_conv(bool on);
 bool deterministic_conv();
 }  // namespace pca
@@ -2482,4 +2484,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("direct_dgrad", &direct_dgrad);
   m.def("direct_wgrad", &direct_wgrad);
   pca::register_comm(m);
+  pca::register_distill(m);
 }

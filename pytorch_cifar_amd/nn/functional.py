@@ -3,6 +3,7 @@ import torch
 import torch.nn.functional as TF
 
 from ..engine import grads
+from ..ops.distill import TopLogits, distill_loss, top_logits  # noqa: F401
 from ..ops.functional import _ref
 from ..ops.functional import (  # noqa: F401
     ChannelSlab,
@@ -29,6 +30,7 @@ from ..ops.functional import (  # noqa: F401
     se_excite,
     split_channels,
     squeeze_excite,
+    unit_grad,
 )
 
 

@@ -1,0 +1,239 @@
+"""Distillation from a teacher's top logits (csrc/distill.hip).
+
+``top_logits`` takes from a teacher's logits what a student's loss needs of them: the k largest of
+each row, their classes, and the row's log-sum-exp. ``distill_loss`` is the loss against that, with
+or without labels. GPU tensors run the native kernels; CPU tensors (and reference mode) take the
+PyTorch path below, whose gradients are autograd's.
+"""
+from __future__ import annotations
+
+import math
+from typing import NamedTuple
+
+import torch
+import torch.nn.functional as F
+
+from .functional import _C, _is_unit, _ref
+
+MAX_CLASSES = 1 << 18
+MAX_K = 1024
+REST = 2.0 ** -20        # csrc/distill.h kDistillRest
+_REDUCTION = {"none": 0, "mean": 1, "sum": 2}
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class TopLogits(NamedTuple):
+    """A teacher's answer: ``values`` [..., k] (descending), ``indices`` [..., k] (int32; a
+    negative one marks an entry that is not kept) and ``lse`` [...] (fp32), the log-sum-exp of all
+    logits / temperature (None where no rest of the mass is wanted)."""
+    values: torch.Tensor
+    indices: torch.Tensor
+    lse: torch.Tensor | None = None
+
+
+def _check_logits(logits, name="logits"):
+    if logits.dim() < 1:
+        raise ValueError(f"{name} must have a class dimension")
+    if logits.dtype not in _FLOATS:
+        raise TypeError(f"{name} must be fp32, bf16 or fp16, got {logits.dtype}")
+    if not 1 <= logits.shape[-1] <= MAX_CLASSES:
+        raise ValueError(f"{name} has {logits.shape[-1]} classes: 1 to {MAX_CLASSES} are supported")
+
+
+def _check_temperature(t):
+    t = float(t)
+    if not (math.isfinite(t) and t > 0):
+        raise ValueError(f"temperature must be positive and finite, got {t}")
+    return t
+
+
+def _rows(x):
+    """[..., n] as [rows, n] whose rows are contiguous in themselves (their stride may be any)."""
+    r = x.reshape(-1, x.shape[-1])
+    if (r.shape[1] > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < 0):
+        r = r.contiguous()
+    return r
+
+
+def top_logits(logits, k, temperature=1.0):
+    """The ``k`` largest logits of each row of ``logits`` [..., classes] as :class:`TopLogits`.
+
+    Descending; among equal logits the lowest class comes first, and NaN counts as the largest.
+    ``lse`` is taken at ``temperature``, that of the loss that will use it; the values are the
+    logits as they are. Not differentiable: a teacher's answer is data to its student.
+    """
+    _check_logits(logits)
+    t = _check_temperature(temperature)
+    n = logits.shape[-1]
+    k = int(k)
+    if not 1 <= k <= min(n, MAX_K):
+        raise ValueError(f"k must be 1 to {min(n, MAX_K)}, got {k}")
+    lead = logits.shape[:-1]
+    with torch.no_grad():
+        if _ref(logits):
+            z = logits.float()
+            values, indices = torch.sort(z, dim=-1, descending=True, stable=True)
+            lse = torch.logsumexp(z.double() / t, -1).float()
+            return TopLogits(values[..., :k].to(logits.dtype), indices[..., :k].to(torch.int32), lse)
+        values, indices, lse = _C().top_logits(_rows(logits.detach()), k, t)
+    return TopLogits(values.view(*lead, k), indices.view(*lead, k), lse.view(lead))
+
+
+def _ref_distill(z, values, indices, lse, target, t, alpha, tail, ignore_index):
+    """The rows' losses in 64 bits, differentiable in ``z`` [rows, classes]."""
+    z = z.double()
+    n, v = z.shape
+    used = (indices >= 0).any(1) if alpha != 0 else torch.zeros(n, dtype=torch.bool, device=z.device)
+    if target is not None and alpha != 1:
+        used = used | (target != ignore_index)
+    z = torch.where(used[:, None], z, torch.zeros_like(z))   # (no term: not looked at)
+    logq = F.log_softmax(z / t, 1)
+    idx = indices.long()
+    kept = idx >= 0
+    bad = (idx >= v).any(1)
+    idx = idx.clamp(0, v - 1)
+    tv = values.double() / t
+    base = (lse.double()[:, None] if tail
+            else torch.logsumexp(tv.masked_fill(~kept, -math.inf), 1, keepdim=True))
+    has = kept.any(1) & (base[:, 0] != -math.inf) & (alpha != 0)
+    live = kept & has[:, None]
+    logp = torch.where(live, tv - base, torch.full_like(tv, -math.inf))
+    p = logp.exp()
+    # (a class without mass takes no part, whatever the student gives it: 0 log 0 = 0)
+    use = live & (p != 0)
+    lq = torch.where(use, logq.gather(1, idx), torch.zeros_like(p))
+    loss = (p * (torch.where(use, logp, torch.zeros_like(p)) - lq)).sum(1)
+    if tail:
+        inside = torch.zeros(n, v + 1, dtype=torch.bool, device=z.device)
+        inside.scatter_(1, torch.where(live, idx, torch.full_like(idx, v)), True)
+        inside = inside[:, :v]
+        rest = 1.0 - p.sum(1)
+        rest = torch.where(has & ~inside.all(1) & ~(rest < REST), rest, torch.zeros_like(rest))
+        some = rest != 0
+        outer = logq.masked_fill(inside, -math.inf)
+        outer = torch.where(some[:, None], outer, torch.zeros_like(outer))
+        lrest = torch.logsumexp(outer, 1)
+        loss = loss + torch.where(some, rest * (torch.where(some, rest, torch.ones_like(rest)).log()
+                                                - lrest), torch.zeros_like(rest))
+    loss = torch.where(has, loss * (alpha * t * t), torch.zeros_like(loss))
+    if target is not None and alpha != 1:
+        hit = target != ignore_index
+        bad = bad | (hit & ((target < 0) | (target >= v)))
+        y = target.clamp(0, v - 1)[:, None]
+        ce = -F.log_softmax(z, 1).gather(1, y)[:, 0]
+        loss = loss + torch.where(hit, (1 - alpha) * ce, torch.zeros_like(ce))
+    return loss * torch.where(bad, math.nan, 1.0).to(loss)
+
+
+class _Distill(torch.autograd.Function):
+    """The forward pass computes the gradient for a unit seed from the row it holds in registers
+    and hands it to the backward, which scales it where the seed is not one. A second backward of
+    a retained graph computes it again from the saved logits."""
+
+    @staticmethod
+    def forward(ctx, z, values, indices, lse, target, cfg):
+        loss, dz = _C().distill(z, values, indices, lse, target, *cfg, True)
+        ctx.save_for_backward(z, values, indices, lse, target)
+        ctx.cfg = cfg
+        ctx.dz = dz
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        saved = ctx.saved_tensors
+        dz, ctx.dz = ctx.dz, None
+        if dz is None:
+            _, dz = _C().distill(*saved, *ctx.cfg, True)
+        if not _is_unit(dloss):
+            _C().scale_rows_(dz, dloss.float().reshape(-1).contiguous())
+        return dz, None, None, None, None, None
+
+
+def distill_loss(logits, top, target=None, temperature=1.0, alpha=None, tail=False,
+                 reduction="mean", ignore_index=-100):
+    """Loss of a student's ``logits`` [..., classes] against a teacher's ``top`` logits.
+
+    With q = softmax(logits / T) a row's loss is
+
+        alpha T^2 KL(p || q) + (1 - alpha) cross_entropy(logits, target)
+
+    ``tail=False``: p is the softmax of the kept teacher logits / T among themselves.
+    ``tail=True``: p is the teacher's own probability of each kept class, exp(value / T - lse), and
+    the mass it leaves to all other classes is one more term, against the mass q leaves to them
+    (``top.lse`` must have been taken at the same T). A rest below 2^-20 counts as none.
+
+    ``target`` [...] holds int64 classes; ``alpha`` defaults to 1 without it and must be given with
+    it. Rows may keep fewer logits (negative indices); a row that keeps none has no teacher term, a
+    row whose target is ``ignore_index`` no label term, and a row with neither is not looked at:
+    loss and gradient 0. ``reduction``: "mean" over all rows, "sum", or "none". A class outside
+    the row makes its loss and gradient NaN.
+
+    Teacher's side is data: gradients flow to ``logits`` alone.
+    """
+    _check_logits(logits)
+    t = _check_temperature(temperature)
+    if reduction not in _REDUCTION:
+        raise ValueError(f"reduction must be one of {sorted(_REDUCTION)}, got {reduction!r}")
+    if alpha is None:
+        if target is not None:
+            raise ValueError("alpha (the weight of the teacher's term) must be given with a target")
+        alpha = 1.0
+    alpha = float(alpha)
+    if not 0 <= alpha <= 1:
+        raise ValueError(f"alpha must be in [0, 1], got {alpha}")
+    if target is None and alpha != 1:
+        raise ValueError("alpha below 1 needs a target")
+    values, indices, lse = top if len(top) == 3 else (*top, None)
+    lead = logits.shape[:-1]
+    k = values.shape[-1] if values.dim() else 0
+    if values.shape[:-1] != lead or indices.shape != values.shape or values.dim() < 1:
+        raise ValueError(f"top values {tuple(values.shape)} and indices {tuple(indices.shape)} do "
+                         f"not fit logits {tuple(logits.shape)}")
+    if not 1 <= k <= MAX_K:
+        raise ValueError(f"1 to {MAX_K} kept logits a row are supported, got {k}")
+    if values.dtype not in _FLOATS or indices.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"top values must be fp32, bf16 or fp16 and indices int32 or int64, got "
+                        f"{values.dtype}, {indices.dtype}")
+    if tail:
+        if lse is None:
+            raise ValueError("tail=True needs the teacher's lse")
+        if lse.shape != lead or lse.dtype != torch.float32:
+            raise ValueError(f"lse must be fp32 of shape {tuple(lead)}")
+    if target is not None and (target.shape != lead or target.dtype != torch.int64):
+        raise ValueError(f"target must be int64 of shape {tuple(lead)}")
+    for name, x in (("values", values), ("indices", indices), ("lse", lse), ("target", target)):
+        if x is not None and x.device != logits.device:
+            raise ValueError(f"{name} is on {x.device}, the logits are on {logits.device}")
+        if x is not None and x.requires_grad:
+            raise ValueError(f"{name} requires grad: a teacher's answer is data, detach it")
+
+    z = _rows(logits)
+    values, indices = values.reshape(-1, k), indices.reshape(-1, k)
+    lse = lse.reshape(-1) if tail else None
+    target = target.reshape(-1) if target is not None else None
+    if _ref(logits):
+        rows = _ref_distill(z, values, indices, lse, target, t, alpha, tail, ignore_index)
+        loss = rows if reduction == "none" else rows.mean() if reduction == "mean" else rows.sum()
+        loss = loss.float()
+    else:
+        from .. import _native
+
+        if _native._debug:   # name a bad class on the host (the kernel NaN-poisons its row)
+            for name, x, low in (("index", indices, None), ("target", target, ignore_index)):
+                if x is None or (name == "target" and alpha == 1):
+                    continue
+                bad = x >= z.shape[1] if low is None else ((x != low) & ((x < 0) | (x >= z.shape[1])))
+                if bool(bad.any()):
+                    at = bad.nonzero()[0].tolist()
+                    raise IndexError(f"distill_loss: {name} {int(x[tuple(at)])} at {at} is outside "
+                                     f"[0, {z.shape[1]})")
+        args = (z, values.contiguous(), indices.contiguous(),
+                lse.contiguous() if tail else None,
+                target.contiguous() if target is not None else None)
+        cfg = (t, alpha, bool(tail), _REDUCTION[reduction], int(ignore_index))
+        if torch.is_grad_enabled() and logits.requires_grad:
+            loss = _Distill.apply(*args, cfg)
+        else:
+            loss, _ = _C().distill(*args, *cfg, False)
+    return loss.view(lead) if reduction == "none" else loss

@@ -1,0 +1,401 @@
+"""The native top_logits / distill_loss kernels against the 64-bit reference path on the CPU.
+
+Tolerances. e_j = exp((z_j - max)/T) has a relative error of at most (3 x + 4) 2^-24, x = |z_j -
+max| / T: one rounding each of the difference, of log2(e)/T and of the product, each worth x 2^-24
+in the exponent, and 2 steps of the exponential instruction. A sum adds one rounding a term that a
+thread holds (at most 256). With x at most X, the row's spread, a sum or a share of it is off by
+at most C = (3 X + 260) 2^-24 relative, the logarithm of a sum by C absolute. The loss holds two
+such logarithms times alpha T^2 and one times 1 - alpha; a gradient element holds shares of them
+times alpha T and 1 - alpha, and is then rounded to its type: half a step, eps / 2 (in fp16 at least
+half of its smallest number, 2^-25).
+"""
+import math
+
+import pytest
+import torch
+
+from pytorch_cifar_amd.nn import functional as PF
+from pytorch_cifar_amd.ops.distill import _ref_distill
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+SIZES = [(3, 1, 1), (1024, 10, 5), (5, 64, 64), (4, 65, 3), (7, 513, 100), (9, 2047, 512),
+         (5, 4097, 17), (3, 8200, 1024), (4, 33001, 256), (2, 50257, 64), (3, 65540, 5),
+         (2, 131072, 64), (2, 262144, 1000)]
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def make(r, v, dtype, seed=0, scale=3.0):
+    g = torch.Generator().manual_seed(seed)
+    return (scale * torch.randn(r, v, generator=g)).to(dtype)
+
+
+def spread(z, t):
+    z = z.double()
+    f = torch.where(torch.isfinite(z), z, torch.zeros_like(z))
+    return ((f.amax() - f.amin()) / min(t, 1.0)).item()
+
+
+def check_top(z, k, t=1.0, gpu=None):
+    want = PF.top_logits(z, k, t)
+    got = PF.top_logits(z.cuda() if gpu is None else gpu, k, t)
+    assert got.indices.dtype == torch.int32 and got.values.dtype == z.dtype
+    assert torch.equal(got.indices.cpu(), want.indices)
+    a, b = got.values.cpu(), want.values
+    assert torch.equal(torch.nan_to_num(a), torch.nan_to_num(b)) and torch.equal(a.isnan(), b.isnan())
+    c = (3 * spread(z, t) + 260) * U
+    lse, ref = got.lse.cpu().double(), torch.logsumexp(z.double() / t, -1)
+    fine = torch.isfinite(ref)
+    assert torch.equal(torch.nan_to_num(lse[~fine]), torch.nan_to_num(ref[~fine]))
+    assert ((lse - ref)[fine].abs() <= c + U * ref[fine].abs()).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("r, v, k", SIZES)
+def test_top_logits(r, v, k, dtype):
+    check_top(make(r, v, dtype), k, 2.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [6, 300, 5000, 40000, 200000])
+def test_top_logits_hard_rows(v, dtype):
+    k = min(v, 200)
+    z = make(12, v, dtype, 1)
+    z[0] = -math.inf
+    z[1] = 1.0                                    # all equal
+    z[2] = torch.randint(0, 3, (v,)).to(dtype)    # few values
+    z[3, v // 2:] = -math.inf
+    z[4, v // 3] = math.nan
+    z[5, 1] = math.inf
+    z[6] = torch.finfo(dtype).min
+    z[7, 3:] = torch.finfo(dtype).min
+    z[8] = torch.where(torch.arange(v) % 2 == 0, 0.0, -0.0).to(dtype)
+    z[9] = torch.arange(v).to(dtype)
+    z[10] = math.nan
+    z[11] = -math.inf
+    z[11, v - 1] = 2.0
+    top = PF.top_logits(z.cuda(), k)
+    want = PF.top_logits(z, k)
+    assert torch.equal(top.indices.cpu(), want.indices)
+    check_top(z[[0, 1, 2, 3, 5, 8, 11]], k)
+    lse = top.lse.cpu()
+    assert lse[0] == -math.inf and lse[5] == math.inf
+    assert lse[4].isnan() and lse[10].isnan()
+    assert abs(lse[11].item() - 2.0) <= 300 * U
+
+
+def test_top_logits_strided_rows():
+    buf = make(9, 1003, torch.bfloat16).cuda()
+    for view in (buf[:, 1:778], buf[::2, 3:500], buf[:, :1], buf[2:3].expand(4, 1003), buf.t()):
+        check_top(view.cpu(), min(view.shape[1], 9), gpu=view)
+
+
+def distill_inputs(r, v, k, dtype, t, seed=3, labels=True):
+    teacher = make(r, v, dtype, seed)
+    z = (0.6 * teacher.float() + make(r, v, torch.float32, seed + 1, 1.5)).to(dtype)
+    top = PF.top_logits(teacher, k, t)
+    y = torch.randint(0, v, (r,), generator=torch.Generator().manual_seed(seed))
+    return z, top, (y if labels else None)
+
+
+def oracle(z, top, y, t, alpha, tail, seeds=None):
+    """Rows' losses and the gradient of (seeds . losses) in 64 bits."""
+    x = z.detach().cpu().double().requires_grad_(True)
+    c = [a.cpu() if a is not None else None for a in (top.values, top.indices, top.lse, y)]
+    loss = _ref_distill(x, *c, t, alpha, tail, -100)
+    w = torch.ones_like(loss) if seeds is None else seeds.double().cpu()
+    (g,) = torch.autograd.grad((loss * w).sum(), x)
+    return loss.detach(), g
+
+
+def tolerances(z, t, alpha, grad, seeds=1.0):
+    z = z.detach().cpu().double()
+    c = (3 * spread(z, t) + 260) * U
+    loss = 2 * c * (alpha * t * t + 1 - alpha)
+    q = alpha * t * torch.softmax(z / t, 1) + (1 - alpha) * torch.softmax(z, 1)
+    return loss, lambda dtype: (2 * c * (q.nan_to_num() + grad.abs()) * seeds
+                                + torch.finfo(dtype).eps / 2 * grad.abs()
+                                + (2.0 ** -25 if dtype == torch.float16 else 1e-37))
+
+
+def gpu_top(top):
+    return PF.TopLogits(*(a.cuda() if a is not None else None for a in top))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("r, v, k", SIZES)
+@pytest.mark.parametrize("tail, labels, t", [(False, True, 4.0), (True, True, 1.0), (True, False, 2.0)])
+def test_distill(r, v, k, dtype, tail, labels, t):
+    alpha = 0.7 if labels else 1.0
+    z, top, y = distill_inputs(r, v, k, dtype, t, labels=labels)
+    if r > 2:
+        top.indices[0, k // 2:] = -1
+        top.indices[2] = -1
+        if labels:
+            y[1] = -100
+            y[2] = -100
+    if k > 2:
+        top.indices[1, 2] = top.indices[1, 0]      # a class twice
+    want, grad = oracle(z, top, y, t, alpha, tail)
+    tl, tg = tolerances(z, t, alpha, grad)
+    x = z.cuda().requires_grad_(True)
+    kw = dict(temperature=t, alpha=alpha, tail=tail)
+    args = (gpu_top(top), y.cuda() if labels else None)
+    rows = PF.distill_loss(x.detach(), *args, reduction="none", **kw)
+    assert ((rows.cpu().double() - want).abs() <= tl + 2 * U * want.abs()).all()
+    loss = PF.distill_loss(x, *args, reduction="sum", **kw)
+    loss.backward(PF.unit_grad(loss))
+    assert abs(loss.item() - rows.double().sum().item()) <= U * rows.double().abs().sum().item() + 1e-30
+    assert x.grad.dtype == dtype
+    assert ((x.grad.cpu().double() - grad).abs() <= tg(dtype)).all()
+    if r > 2 and labels:
+        assert (x.grad[2] == 0).all() and rows[2] == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_reductions_and_seeds(dtype):
+    r, v, k, t = 6, 777, 9, 2.0
+    z, top, y = distill_inputs(r, v, k, dtype, t)
+    seeds = torch.tensor([1.0, 0.0, -2.5, 0.125, 1.0, 3.0])
+    kw = dict(temperature=t, alpha=0.5, tail=True)
+    args = (gpu_top(top), y.cuda())
+    x = z.cuda().requires_grad_(True)
+    _, grad = oracle(z, top, y, t, 0.5, True, seeds)
+    _, tg = tolerances(z, t, 0.5, grad, 1 + seeds.abs()[:, None].double())
+    loss = PF.distill_loss(x, *args, reduction="none", **kw)
+    (g,) = torch.autograd.grad(loss, x, seeds.cuda())
+    # (the factor is applied to a gradient that was rounded before: a second half step)
+    half = torch.finfo(dtype).eps / 2
+    extra = half * grad.abs() + (2.0 ** -23 if dtype == torch.float16 else 0)
+    assert ((g.cpu().double() - grad).abs() <= tg(dtype) + extra).all()
+    # the mean, by another seed, twice over a retained graph
+    _, one = oracle(z, top, y, t, 0.5, True, torch.full((r,), 3.0 / r))
+    _, tg = tolerances(z, t, 0.5, one)
+    loss = PF.distill_loss(x, *args, **kw)
+    seed = torch.tensor(3.0, device="cuda")
+    a = torch.autograd.grad(loss, x, seed, retain_graph=True)[0]
+    a0 = a.clone()
+    a.add_(1.0)                       # what a caller does to its gradient is its own affair
+    b = torch.autograd.grad(loss, x, seed)[0]
+    assert torch.equal(a0, b)
+    extra = half * one.abs() + (2.0 ** -23 if dtype == torch.float16 else 0)
+    assert ((b.cpu().double() - one).abs() <= tg(dtype) + extra).all()
+
+
+def test_gradient_matches_differences():
+    z, top, y = distill_inputs(3, 40, 7, torch.float32, 2.0)
+    kw = dict(temperature=2.0, alpha=0.6, tail=True, reduction="sum")
+    x = z.cuda().requires_grad_(True)
+    PF.distill_loss(x, gpu_top(top), y.cuda(), **kw).backward()
+    ref = lambda d: _ref_distill(d, *top, y, 2.0, 0.6, True, -100).sum().item()   # noqa: E731
+    h = 1e-4
+    c = (3 * spread(z, 2.0) + 260) * U
+    for i in range(3):
+        for j in range(0, 40, 3):
+            d = torch.zeros(3, 40, dtype=torch.float64)
+            d[i, j] = h
+            fd = (ref(z.double() + d) - ref(z.double() - d)) / (2 * h)
+            # h^2 / 6 times a third derivative below 1, and the kernel's own C
+            assert abs(x.grad[i, j].item() - fd) <= h * h + 8 * c
+
+
+def test_strides_types_and_shapes():
+    z, top, y = distill_inputs(12, 515, 20, torch.float32, 1.0)
+    big = torch.full((12, 1031), math.nan)
+    big[:, 3:518] = z
+    big = big.cuda()
+    kw = dict(alpha=0.5, tail=True, reduction="none")
+    base = PF.distill_loss(z.cuda(), gpu_top(top), y.cuda(), **kw)
+    assert torch.equal(PF.distill_loss(big[:, 3:518], gpu_top(top), y.cuda(), **kw), base)
+    assert torch.equal(PF.distill_loss(z.cuda().t().contiguous().t(), gpu_top(top), y.cuda(), **kw), base)
+    T = PF.TopLogits
+    g = gpu_top(top)
+    assert torch.equal(PF.distill_loss(z.cuda(), T(g.values, g.indices.long(), g.lse), y.cuda(), **kw), base)
+    wide = torch.cat([g.values, g.values], 1)[:, :20]
+    assert torch.equal(PF.distill_loss(z.cuda(), T(wide, g.indices, g.lse), y.cuda(), **kw), base)
+    half = T(g.values.bfloat16(), g.indices, g.lse)
+    same = T(half.values.float(), g.indices, g.lse)
+    assert torch.equal(PF.distill_loss(z.cuda(), half, y.cuda(), **kw),
+                       PF.distill_loss(z.cuda(), same, y.cuda(), **kw))
+    nd = PF.distill_loss(z.cuda().view(3, 4, 515), T(g.values.view(3, 4, 20), g.indices.view(3, 4, 20),
+                                                     g.lse.view(3, 4)), y.cuda().view(3, 4), **kw)
+    assert torch.equal(nd, base.view(3, 4))
+    x = big.clone().requires_grad_(True)
+    PF.distill_loss(x[:, 3:518], g, y.cuda(), alpha=0.5, tail=True).backward()
+    assert (x.grad[:, :3] == 0).all() and (x.grad[:, 518:] == 0).all()
+    assert torch.isfinite(x.grad).all() and (x.grad[:, 3:518] != 0).any()
+
+
+def test_masked_classes_and_empty_rows():
+    """Classes masked by -inf or the type's lowest value; rows without terms may hold anything."""
+    for dtype in DTYPES:
+        z, top, y = distill_inputs(8, 300, 6, dtype, 1.0)
+        teacher = make(8, 300, dtype, 3)
+        teacher[:, 200:] = -math.inf
+        top = PF.top_logits(teacher, 6)
+        y = top.indices[:, 1].long()
+        low = torch.finfo(dtype).min
+        z[0, 200:] = -math.inf
+        z[1, 200:] = low
+        z[2] = math.nan
+        top.indices[2], y[2] = -1, -100
+        z[3] = -math.inf
+        top.indices[3], y[3] = -1, -100
+        z[4] = low                                    # uniform
+        top.values[5] = -math.inf                     # a teacher's row of no mass
+        top.lse[5] = -math.inf
+        y[5] = -100
+        z[6, 7] = math.nan
+        rows = {}
+        for tail in (False, True):
+            x = z.cuda().requires_grad_(True)
+            loss = PF.distill_loss(x, gpu_top(top), y.cuda(), alpha=0.5, tail=tail, reduction="none")
+            loss.backward(torch.ones_like(loss))
+            want, grad = oracle(z, top, y, 1.0, 0.5, tail)
+            keep = [0, 1, 4, 7]
+            tl, tg = tolerances(z[[0, 7]], 1.0, 0.5, grad[[0, 7]])
+            assert ((loss.cpu().double() - want).abs()[keep] <= tl + 2 * U * want.abs()[keep]).all()
+            assert ((x.grad.cpu().double() - grad).abs()[[0, 7]] <= tg(dtype)).all()
+            # a row of one value has q = 1/300 everywhere: shares without rounding of a spread
+            assert ((x.grad.cpu().double() - grad).abs()[4] <= torch.finfo(dtype).eps
+                    * (grad[4].abs() + 1 / 300) + 2.0 ** -25).all()
+            assert (x.grad[1, 200:] == 0).all()
+            for i in (2, 3, 5):
+                assert loss[i] == 0 and (x.grad[i] == 0).all()
+            assert loss[6].isnan()
+            rows[tail] = loss.detach()
+        assert torch.isfinite(rows[False][keep]).all()
+
+
+def test_bad_classes_poison_their_row():
+    z, top, y = distill_inputs(4, 50, 3, torch.float32, 1.0)
+    top.indices[1, 0], y[2], y[3] = 50, 50, -7
+    x = z.cuda().requires_grad_(True)
+    loss = PF.distill_loss(x, gpu_top(top), y.cuda(), alpha=0.5, reduction="none")
+    loss.backward(torch.ones_like(loss))
+    assert loss.isnan().tolist() == [False, True, True, True]
+    assert x.grad.isnan().all(1).tolist() == [False, True, True, True]
+
+
+def test_debug_mode_names_a_bad_class():
+    import pytorch_cifar_amd as pca
+
+    z, top, y = distill_inputs(4, 50, 3, torch.float32, 1.0)
+    top.indices[1, 2] = 50
+    pca.set_debug_sync(True)
+    try:
+        with pytest.raises(IndexError, match="50"):
+            PF.distill_loss(z.cuda(), gpu_top(top))
+    finally:
+        pca.set_debug_sync(False)
+
+
+def test_no_rows():
+    top = PF.top_logits(torch.zeros(0, 33, device="cuda"), 4)
+    assert top.values.shape == (0, 4)
+    x = torch.zeros(0, 33, device="cuda", requires_grad=True)
+    loss = PF.distill_loss(x, top, reduction="sum")
+    loss.backward()
+    assert loss.item() == 0 and x.grad.shape == (0, 33)
+    assert PF.distill_loss(x, top).isnan()
+
+
+def test_other_stream_and_same_bits():
+    z, top, y = distill_inputs(64, 5003, 50, torch.bfloat16, 2.0)
+    x, g, yc = z.cuda().requires_grad_(True), gpu_top(top), y.cuda()
+    torch.cuda.synchronize()
+
+    def both():
+        loss = PF.distill_loss(x, g, yc, temperature=2.0, alpha=0.5, tail=True)
+        return (loss.detach(), *torch.autograd.grad(loss, x), *PF.top_logits(x, 50, 2.0))
+
+    first = both()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        second = both()
+    s.synchronize()
+    third = both()
+    for a, b, c in zip(first, second, third):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_captured_and_replayed():
+    """The teacher's selection, the loss and its gradient in one graph, replayed over new logits with
+    eager work between; each replay against the eager result, bit by bit."""
+    dev = "cuda"
+    t = torch.empty(32, 1000, device=dev)
+    z = torch.empty(32, 1000, device=dev)
+    y = torch.empty(32, dtype=torch.int64, device=dev)
+
+    def fill(seed):
+        g = torch.Generator(device=dev).manual_seed(seed)
+        t.copy_(3 * torch.randn(32, 1000, generator=g, device=dev))
+        z.copy_(2 * torch.randn(32, 1000, generator=g, device=dev))
+        y.copy_(torch.randint(0, 1000, (32,), generator=g, device=dev))
+
+    def step():
+        x = z.detach().requires_grad_(True)
+        loss = PF.distill_loss(x, PF.top_logits(t, 20, 2.0), y, temperature=2.0, alpha=0.5, tail=True)
+        (d,) = torch.autograd.grad(loss, x, PF.unit_grad(loss))
+        return loss.detach(), d
+
+    fill(0)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graphs = []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = step()
+        graphs.append((gr, out))
+    for i in range(6):
+        fill(10 + i)
+        want = step()
+        gr, out = graphs[i % 2]
+        gr.replay()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+
+
+def test_offsets_past_32_bits():
+    r, v, k = 17000, 131072, 3
+    z = torch.zeros(r, v, dtype=torch.bfloat16, device="cuda")
+    z[-1] = make(1, v, torch.bfloat16).cuda()[0]
+    top = PF.top_logits(z, k)
+    want = PF.top_logits(z[-1:].cpu(), k)
+    assert torch.equal(top.indices[-1:].cpu(), want.indices)
+    assert top.indices[:-1].cpu().tolist() == [[0, 1, 2]] * (r - 1)
+    x = z.requires_grad_(True)
+    loss = PF.distill_loss(x, top, reduction="sum")
+    (d,) = torch.autograd.grad(loss, x)
+    last = x.detach()[-1:].cpu()
+    _, grad = oracle(last, want, None, 1.0, 1.0, False)
+    _, tg = tolerances(last, 1.0, 1.0, grad)
+    assert ((d[-1:].cpu().double() - grad).abs() <= tg(torch.bfloat16)).all()
+    assert torch.equal(d[0], d[-2])
+
+
+def test_refusals_on_the_gpu():
+    z, top, y = distill_inputs(4, 50, 3, torch.float32, 1.0)
+    g = gpu_top(top)
+    with pytest.raises(ValueError):
+        PF.distill_loss(z.cuda(), top)                       # the teacher's side on the host
+    with pytest.raises(ValueError):
+        PF.distill_loss(z.cuda(), g, y, alpha=0.5)
+    with pytest.raises(ValueError):
+        PF.top_logits(z.cuda(), 51)
+    from pytorch_cifar_amd import _native
+
+    C = _native.lib()
+    with pytest.raises(RuntimeError):
+        C.top_logits(z.cuda().t(), 1, 1.0)                   # classes not contiguous
+    with pytest.raises(RuntimeError):
+        C.top_logits(z, 1, 1.0)
+    with pytest.raises(RuntimeError):
+        C.distill(z.cuda(), g.values[:, ::2], g.indices[:, ::2], None, None, 1.0, 1.0, False, 1, -100, True)
+    with pytest.raises(RuntimeError):
+        C.distill(z.cuda(), g.values, g.indices, None, None, 1.0, 1.0, True, 1, -100, True)
