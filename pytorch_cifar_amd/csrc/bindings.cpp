@@ -244,6 +244,8 @@ void direct_wgrad_launch(const bf16*, const bf16*, int, int, int, int, int, int,
 void register_comm(py::module& m);
 // bindings_distill.cpp
 void register_distill(py::module& m);
+// bindings_gated.cpp
+void register_gated(py::module& m);
 void set_deterministic_conv(bool on);
 bool deterministic_conv();
 }  // namespace pca
@@ -2485,4 +2487,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("direct_wgrad", &direct_wgrad);
   pca::register_comm(m);
   pca::register_distill(m);
+  pca::register_gated(m);
 }

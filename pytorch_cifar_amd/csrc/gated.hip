@@ -1,0 +1,482 @@
+// Gated linear layer: h = act(x Wg^T) * (x Wu^T) and its gradients.
+//
+// Three products run on one tiled kernel, each with fp32 sums on the matrix cores:
+//   forward  both projections of a tile of hidden units in one pass over x, the activation and the
+//            product in the epilogue (the projections never leave the registers, but for the fp32
+//            copies that a backward pass wants);
+//   dX       [dg | du] times [Wg; Wu], one sum over both halves;
+//   dW       [dg | du]^T x.
+// dg = dh u act'(g) and du = dh act(g) are formed from the fp32 projections and rounded once to the
+// operands' type.
+#include "gated.h"
+#include "mfma_util.h"
+
+#include <algorithm>
+
+namespace pca {
+namespace {
+
+typedef _Float16 f16;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// -------------------------------------------------------------------------- matrix fragments
+// A K step takes 64 bytes of each row: 32 16-bit or 16 fp32 terms. A lane holds 16 bytes of it:
+// row (lane & 15), piece (lane >> 4). mma() sums over the step into a 16 x 16 tile: lane l gets
+// column (l & 15) of the second operand and rows 4 (l >> 4) .. + 3 of the first.
+template <typename E>
+struct Mat;
+
+template <>
+struct Mat<bf16> {
+  typedef bf16x8 frag;
+  static __device__ __forceinline__ void mma(const frag& a, const frag& b, f32x4& c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mat<f16> {
+  typedef f16x8 frag;
+  static __device__ __forceinline__ void mma(const frag& a, const frag& b, f32x4& c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mat<float> {
+  typedef f32x4 frag;
+  // instruction e sums over element e of the four lane groups' pieces: terms e, 4 + e, 8 + e, 12 + e
+  static __device__ __forceinline__ void mma(const frag& a, const frag& b, f32x4& c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+  }
+};
+
+constexpr int kRow = 128;   // bytes of a row that a K tile takes: 64 16-bit or 32 fp32 terms
+template <typename E>
+constexpr int kBK = kRow / (int)sizeof(E);
+template <typename E>
+constexpr int kPiece = 16 / (int)sizeof(E);   // elements of 16 bytes
+
+// LDS images of a K tile; both are written by 1-KiB DMA pieces, whose lanes choose the address they
+// read so that the bytes land swizzled.
+//   rows:  [tile row][128 bytes of its terms], 16-byte piece c of row r at c ^ (r & 7): the 16 rows
+//          of a fragment read spread over all banks.
+//   terms: operands whose terms are their rows. Blocks of [term][256 bytes of columns], read
+//          transposed (16-bit: ds_read_b64_tr; fp32: four reads of 4 bytes).
+template <typename E>
+__device__ __forceinline__ typename Mat<E>::frag frag_rows(const char* lds, int r0, int s, int lane) {
+  const int r = r0 + (lane & 15), c = 4 * s + (lane >> 4);
+  return *reinterpret_cast<const typename Mat<E>::frag*>(lds + r * kRow + ((c ^ (r & 7)) << 4));
+}
+
+template <typename E>
+__device__ __forceinline__ int swz_terms(int term) {
+  if constexpr (sizeof(E) == 2) return tr_swz<256>(term);
+  else return ((term >> 2) & 3) << 2;
+}
+
+template <typename E>
+__device__ __forceinline__ typename Mat<E>::frag frag_terms(const char* lds, int c0, int s, int lane) {
+  constexpr int kCols = 256 / (int)sizeof(E);        // columns of a block
+  const char* blk = lds + (c0 / kCols) * (kBK<E> * 256);
+  if constexpr (sizeof(E) == 2) {
+    return __builtin_bit_cast(typename Mat<E>::frag, tr_frag<128>(blk, 32 * s, c0 % kCols, lane));
+  } else {
+    f32x4 v;
+    const int col = c0 % kCols + (lane & 15);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int k = 16 * s + 4 * (lane >> 4) + e;
+      v[e] = *reinterpret_cast<const float*>(
+          blk + k * 256 + (((col >> 2) ^ swz_terms<float>(k)) << 4) + ((col & 3) << 2));
+    }
+    return v;
+  }
+}
+
+__device__ __forceinline__ float act_val(float g, int act) { return apply_act(g, act); }
+
+// 4 consecutive outputs of a row at column n (N columns in all), at any alignment
+template <typename O>
+__device__ __forceinline__ void store4(O* row, int n, int N, const f32x4& v) {
+  O h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = static_cast<O>(v[i]);
+  if (n + 4 <= N) {
+    __builtin_memcpy(row + n, h, sizeof(h));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < N) row[n + i] = h[i];
+  }
+}
+
+// ---------------------------------------------------------------------------- tiled product
+template <typename E, typename O, int FORM, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM* WN * 64) void gated_kernel(GatedArgs a, int mt, int nt) {
+  constexpr int NW = WM * WN, NT = NW * 64;
+  constexpr int TM = BM / WM, TN = BN / WN;          // a wave's tile
+  constexpr int MF = TM / 16, NF = TN / 16;
+  constexpr bool kFwd = FORM == GATED_FWD;
+  constexpr bool kTermsQ = FORM == GATED_DW, kTermsP = FORM != GATED_FWD;
+  constexpr int BK = kBK<E>, ES = sizeof(E), PC = kPiece<E>;
+  constexpr int QB = BM * kRow, PB = BN * kRow;      // bytes of a K tile
+  constexpr int QP = QB / 1024 / NW, PP = PB / 1024 / NW;   // DMA pieces of a wave
+  static_assert(QB % (1024 * NW) == 0 && PB % (1024 * NW) == 0, "whole pieces a wave");
+  __shared__ __attribute__((aligned(1024))) char lds[2][QB + PB];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  // consecutive workgroups of an XCD walk M first within a group of 8 N tiles
+  const int wg = xcd_remap(blockIdx.x, gridDim.x);
+  constexpr int G = 8;
+  const int per = G * mt, grp = wg / per, first = grp * G, gn = min(G, nt - first);
+  const int ni = first + (wg % per) % gn, mi0 = (wg % per) / gn;
+  int half = 0, mi = mi0;
+  if constexpr (FORM == GATED_DW) {
+    half = mi0 >= mt / 2;
+    mi = half ? mi0 - mt / 2 : mi0;
+  }
+  constexpr int NH = kFwd ? BN / 2 : BN;             // output columns of a tile
+  const int m0 = mi * BM, n0 = ni * NH;
+
+  const int per_seg = (a.K + BK - 1) / BK;
+  const int nk = FORM == GATED_DX ? 2 * per_seg : per_seg;
+  const int split = blockIdx.y;
+  const int t0 = (int)((int64_t)nk * split / gridDim.y);
+  const int t1 = (int)((int64_t)nk * (split + 1) / gridDim.y);
+
+  // ---- where each lane's pieces come from, relative to a base that moves with the K tile
+  uint32_t qoff[QP], poff[PP];
+  int qk[QP], pk[PP];                                // first term of the piece in its K tile
+#pragma unroll
+  for (int i = 0; i < QP; ++i) {
+    const int p = i * NW + wave;
+    if constexpr (kTermsQ) {
+      const int term = (p * 4 + (lane >> 4)) % BK, blk = p * 4 / BK;
+      const int c = blk * (256 / ES) + (((lane & 15) ^ swz_terms<E>(term)) * PC);
+      qk[i] = term;
+      qoff[i] = m0 + c < a.mcols ? (uint32_t)(term * a.ldq + c) * ES : kOOB;
+    } else {
+      const int r = p * 8 + (lane >> 3), c = ((lane & 7) ^ (r & 7)) * PC;
+      qk[i] = c;
+      qoff[i] = m0 + r < a.M ? (uint32_t)(r * a.ldq + c) * ES : kOOB;
+    }
+  }
+  bool up[PP];                                       // (wave-uniform: a piece is 8 rows of one half)
+#pragma unroll
+  for (int i = 0; i < PP; ++i) {
+    const int p = i * NW + wave;
+    up[i] = false;
+    if constexpr (kTermsP) {
+      const int term = (p * 4 + (lane >> 4)) % BK, blk = p * 4 / BK;
+      const int c = blk * (256 / ES) + (((lane & 15) ^ swz_terms<E>(term)) * PC);
+      pk[i] = term;
+      poff[i] = n0 + c < a.ncols ? (uint32_t)(term * a.ldp + c) * ES : kOOB;
+    } else {
+      // a wave's TN rows: TN/2 of the gate, then the same TN/2 hidden units of the other
+      const int r = p * 8 + (lane >> 3), c = ((lane & 7) ^ (r & 7)) * PC;
+      const int rw = (p * 8) / TN, rq = r % TN;
+      up[i] = (p * 8) % TN >= TN / 2;
+      const int f = rw * (TN / 2) + rq % (TN / 2);
+      pk[i] = c;
+      poff[i] = n0 + f < a.N ? (uint32_t)(f * a.ldp + c) * ES : kOOB;
+    }
+  }
+  const char* qb = reinterpret_cast<const char*>(a.q);
+  if constexpr (kTermsQ) qb += ((int64_t)half * a.qseg + m0) * ES;
+  else qb += (int64_t)m0 * a.ldq * ES;
+
+  auto issue = [&](int t, int buf) {
+    const int seg = FORM == GATED_DX && t >= per_seg;
+    const int k0 = (t - (seg ? per_seg : 0)) * BK;
+    const char* q = qb + (kTermsQ ? (int64_t)k0 * a.ldq : (int64_t)k0 + seg * a.qseg) * ES;
+    const auto rq = make_rsrc(q, 0x7fffffffu);
+#pragma unroll
+    for (int i = 0; i < QP; ++i)
+      dma16(rq, &lds[buf][(i * NW + wave) * 1024], k0 + qk[i] < a.K ? qoff[i] : kOOB);
+    if constexpr (kFwd) {
+      const char* g = reinterpret_cast<const char*>(a.p0) + ((int64_t)n0 * a.ldp + k0) * ES;
+      const char* u = reinterpret_cast<const char*>(a.p1) + ((int64_t)n0 * a.ldp + k0) * ES;
+#pragma unroll
+      for (int i = 0; i < PP; ++i)
+        dma16(make_rsrc(up[i] ? u : g, 0x7fffffffu), &lds[buf][QB + (i * NW + wave) * 1024],
+              k0 + pk[i] < a.K ? poff[i] : kOOB);
+    } else {
+      const char* p = reinterpret_cast<const char*>(seg ? a.p1 : a.p0) +
+                      ((int64_t)k0 * a.ldp + n0) * ES;
+      const auto rp = make_rsrc(p, 0x7fffffffu);
+#pragma unroll
+      for (int i = 0; i < PP; ++i)
+        dma16(rp, &lds[buf][QB + (i * NW + wave) * 1024], k0 + pk[i] < a.K ? poff[i] : kOOB);
+    }
+  };
+
+  f32x4 acc[NF][MF];
+#pragma unroll
+  for (int i = 0; i < NF; ++i)
+#pragma unroll
+    for (int j = 0; j < MF; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
+
+  if (t0 < t1) issue(t0, 0);
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    if (t + 1 < t1) {
+      issue(t + 1, buf ^ 1);
+      wait_vmcnt<QP + PP>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    raw_barrier();
+    const char* lq = lds[buf];
+    const char* lp = lds[buf] + QB;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      typename Mat<E>::frag q[MF], p[NF];
+#pragma unroll
+      for (int j = 0; j < MF; ++j)
+        q[j] = kTermsQ ? frag_terms<E>(lq, wm * TM + 16 * j, s, lane)
+                       : frag_rows<E>(lq, wm * TM + 16 * j, s, lane);
+#pragma unroll
+      for (int i = 0; i < NF; ++i)
+        p[i] = kTermsP ? frag_terms<E>(lp, wn * TN + 16 * i, s, lane)
+                       : frag_rows<E>(lp, wn * TN + 16 * i, s, lane);
+#pragma unroll
+      for (int i = 0; i < NF; ++i)
+#pragma unroll
+        for (int j = 0; j < MF; ++j) Mat<E>::mma(p[i], q[j], acc[i][j]);
+    }
+    // every wave has its fragments before the buffer is written again
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    raw_barrier();
+  }
+
+  // ---- epilogue: lane holds columns 4 (lane >> 4) .. + 3 of row (lane & 15) of each 16 x 16 tile
+  const int cl = 4 * (lane >> 4);
+  if constexpr (kFwd) {
+#pragma unroll
+    for (int j = 0; j < MF; ++j) {
+      const int m = m0 + wm * TM + 16 * j + (lane & 15);
+      if (m >= a.M) continue;
+#pragma unroll
+      for (int i = 0; i < NF / 2; ++i) {
+        const int n = n0 + wn * (TN / 2) + 16 * i + cl;
+        const f32x4 g = acc[i][j], u = acc[i + NF / 2][j];
+        if (a.part) {
+          float* row = a.part + ((int64_t)split * a.M + m) * 2 * a.N;
+          store4(row, n, a.N, g);
+          store4(row + a.N, n, a.N, u);
+          continue;
+        }
+        f32x4 h;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = act_val(g[e], a.act) * u[e];
+        store4(reinterpret_cast<O*>(a.out0) + (int64_t)m * a.N, n, a.N, h);
+        if (a.save_g) {
+          store4(a.save_g + (int64_t)m * a.N, n, a.N, g);
+          store4(a.save_u + (int64_t)m * a.N, n, a.N, u);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < MF; ++j) {
+      const int m = m0 + wm * TM + 16 * j + (lane & 15);
+      if (m >= a.M) continue;
+#pragma unroll
+      for (int i = 0; i < NF; ++i) {
+        const int n = n0 + wn * TN + 16 * i + cl;
+        if (a.part) {
+          const int64_t rows = (FORM == GATED_DW ? 2 : 1) * (int64_t)a.M;
+          store4(a.part + (split * rows + half * (int64_t)a.M + m) * a.N, n, a.N, acc[i][j]);
+        } else {
+          O* out = reinterpret_cast<O*>(half ? a.out1 : a.out0);
+          store4(out + (int64_t)m * a.N, n, a.N, acc[i][j]);
+        }
+      }
+    }
+  }
+}
+
+// Sums of the K splits, in order, and the epilogue that follows them.
+template <typename O, int FORM>
+__global__ __launch_bounds__(256) void gated_join_kernel(GatedArgs a, int64_t n) {
+  const int64_t total = FORM == GATED_FWD || FORM == GATED_DW ? 2 * n : n;   // floats of a split
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    if constexpr (FORM == GATED_FWD) {
+      const int64_t m = i / a.N, f = i % a.N;
+      float g = 0.f, u = 0.f;
+      for (int s = 0; s < a.splits; ++s) {
+        const float* row = a.part + s * total + m * 2 * a.N;
+        g += row[f];
+        u += row[a.N + f];
+      }
+      reinterpret_cast<O*>(a.out0)[i] = static_cast<O>(act_val(g, a.act) * u);
+      if (a.save_g) {
+        a.save_g[i] = g;
+        a.save_u[i] = u;
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < (FORM == GATED_DW ? 2 : 1); ++h) {
+        float v = 0.f;
+        for (int s = 0; s < a.splits; ++s) v += a.part[s * total + h * n + i];
+        reinterpret_cast<O*>(h ? a.out1 : a.out0)[i] = static_cast<O>(v);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------ elementwise passes
+template <typename E>
+__global__ __launch_bounds__(256) void gated_dact_kernel(const float* __restrict__ g,
+                                                         const float* __restrict__ u,
+                                                         const E* __restrict__ dh, int64_t lddh,
+                                                         int64_t M, int F, int Fp, int act,
+                                                         E* __restrict__ out) {
+  constexpr int PC = kPiece<E>;
+  const int pieces = Fp / PC;
+  for (int64_t w = blockIdx.x * 256ll + threadIdx.x; w < M * pieces; w += (int64_t)gridDim.x * 256) {
+    const int64_t m = w / pieces;
+    const int f0 = (int)(w % pieces) * PC;
+    E dg[PC], du[PC];
+    float gv[PC], uv[PC];
+    E d[PC];
+    if (f0 + PC <= F) {
+      __builtin_memcpy(gv, g + m * F + f0, sizeof(gv));
+      __builtin_memcpy(uv, u + m * F + f0, sizeof(uv));
+      __builtin_memcpy(d, dh + m * lddh + f0, sizeof(d));
+    } else {
+#pragma unroll
+      for (int i = 0; i < PC; ++i) {
+        const bool in = f0 + i < F;
+        gv[i] = in ? g[m * F + f0 + i] : 0.f;
+        uv[i] = in ? u[m * F + f0 + i] : 0.f;
+        d[i] = in ? dh[m * lddh + f0 + i] : static_cast<E>(0.f);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PC; ++i) {
+      const float df = static_cast<float>(d[i]);
+      dg[i] = static_cast<E>(df * uv[i] * act_grad(gv[i], act));
+      du[i] = static_cast<E>(df * act_val(gv[i], act));
+    }
+    E* row = out + m * 2 * Fp + f0;
+    __builtin_memcpy(row, dg, 16);
+    __builtin_memcpy(row + Fp, du, 16);
+  }
+}
+
+template <typename S, typename E>
+__global__ __launch_bounds__(256) void gated_operand_kernel(const S* __restrict__ src, int64_t ld,
+                                                            int64_t R, int n, E* __restrict__ dst,
+                                                            int np) {
+  constexpr int PC = kPiece<E>;
+  const int pieces = np / PC;
+  for (int64_t w = blockIdx.x * 256ll + threadIdx.x; w < R * pieces; w += (int64_t)gridDim.x * 256) {
+    const int64_t r = w / pieces;
+    const int c = (int)(w % pieces) * PC;
+    E v[PC];
+    if (c + PC <= n) {
+      S s[PC];
+      __builtin_memcpy(s, src + r * ld + c, sizeof(s));
+#pragma unroll
+      for (int i = 0; i < PC; ++i) v[i] = static_cast<E>(static_cast<float>(s[i]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < PC; ++i)
+        v[i] = static_cast<E>(c + i < n ? static_cast<float>(src[r * ld + c + i]) : 0.f);
+    }
+    __builtin_memcpy(dst + r * np + c, v, 16);
+  }
+}
+
+template <typename F>
+void pick_type(int type, F&& fn) {
+  if (type == GATED_F32) fn(float());
+  else if (type == GATED_BF16) fn(bf16());
+  else fn(f16());
+}
+
+uint32_t grid_for(int64_t n) { return (uint32_t)std::max<int64_t>(1, std::min<int64_t>((n + 255) / 256, 4096)); }
+
+constexpr int kCUs = 256;
+
+// 256 x 256 tiles where they fill the card at least once, 128 x 128 ones below
+struct Plan {
+  bool big;
+  int mt, nt, splits;
+};
+Plan plan(int form, int type, int M, int N, int K) {
+  Plan p{};
+  const int halves = form == GATED_DW ? 2 : 1, nh = form == GATED_FWD ? 2 : 1;
+  auto tiles = [&](int b) { return (int64_t)halves * cdiv(M, b) * cdiv(N * nh, b); };
+  p.big = tiles(256) >= kCUs;
+  const int b = p.big ? 256 : 128;
+  p.mt = halves * cdiv(M, b);
+  p.nt = cdiv(N * nh, b);
+  const int nk = (form == GATED_DX ? 2 : 1) * cdiv(K, 128 / (type == GATED_F32 ? 4 : 2));
+  const int64_t t = (int64_t)p.mt * p.nt;
+  // few tiles: the sum is split until the card is filled once, to no less than 4 K tiles each
+  p.splits = 1;
+  if (t * 2 <= kCUs) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kCUs / t, nk / 4));
+  return p;
+}
+
+}  // namespace
+
+int gated_splits(int form, int type, int M, int N, int K) { return plan(form, type, M, N, K).splits; }
+
+int64_t gated_part_floats(int form, int M, int N) {
+  return (int64_t)M * N * (form == GATED_DX ? 1 : 2);
+}
+
+void gated_launch(int form, int type, bool out_f32, const GatedArgs& a, hipStream_t st) {
+  const Plan p = plan(form, type, a.M, a.N, a.K);
+  const dim3 grid((uint32_t)(p.mt * p.nt), (uint32_t)a.splits);
+  const int64_t n = (int64_t)a.M * a.N;
+  auto go = [&](auto ev, auto ov, auto fv) {
+    using E = decltype(ev);
+    using O = decltype(ov);
+    constexpr int FORM = decltype(fv)::value;
+    if (p.big)
+      hipLaunchKernelGGL((gated_kernel<E, O, FORM, 256, 256, 2, 4>), grid, dim3(512), 0, st, a, p.mt, p.nt);
+    else
+      hipLaunchKernelGGL((gated_kernel<E, O, FORM, 128, 128, 2, 2>), grid, dim3(256), 0, st, a, p.mt, p.nt);
+    if (a.part)
+      hipLaunchKernelGGL((gated_join_kernel<O, FORM>), dim3(grid_for(n)), dim3(256), 0, st, a, n);
+  };
+  pick_type(type, [&](auto ev) {
+    using E = decltype(ev);
+    using std::integral_constant;
+    if (form == GATED_FWD) go(ev, ev, integral_constant<int, GATED_FWD>());
+    else if (form == GATED_DX) go(ev, ev, integral_constant<int, GATED_DX>());
+    else if (out_f32) go(ev, float(), integral_constant<int, GATED_DW>());
+    else go(ev, ev, integral_constant<int, GATED_DW>());
+  });
+}
+
+void gated_dact_launch(int type, const float* g, const float* u, const void* dh, int64_t lddh,
+                       int64_t M, int F, int Fp, int act, void* dgdu, hipStream_t st) {
+  pick_type(type, [&](auto ev) {
+    using E = decltype(ev);
+    hipLaunchKernelGGL((gated_dact_kernel<E>), dim3(grid_for(M * (Fp / kPiece<E>))), dim3(256), 0,
+                       st, g, u, reinterpret_cast<const E*>(dh), lddh, M, F, Fp, act,
+                       reinterpret_cast<E*>(dgdu));
+  });
+}
+
+void gated_operand_launch(const void* src, int src_type, int64_t ld, int64_t R, int n, void* dst,
+                          int dst_type, int np, hipStream_t st) {
+  pick_type(src_type, [&](auto sv) {
+    pick_type(dst_type, [&](auto ev) {
+      using S = decltype(sv);
+      using E = decltype(ev);
+      hipLaunchKernelGGL((gated_operand_kernel<S, E>), dim3(grid_for(R * (np / kPiece<E>))),
+                         dim3(256), 0, st, reinterpret_cast<const S*>(src), ld, R, n,
+                         reinterpret_cast<E*>(dst), np);
+    });
+  });
+}
+
+}  // namespace pca

@@ -1,2 +1,3 @@
 from . import functional  # noqa: F401
-from .modules import AvgPool2d, BatchNorm2d, Conv2d, Linear, MaxPool2d, ReLU, Sequential  # noqa: F401
+from .modules import (AvgPool2d, BatchNorm2d, Conv2d, GatedLinear, Linear, MaxPool2d,  # noqa: F401
+                      ReLU, Sequential)

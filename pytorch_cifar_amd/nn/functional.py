@@ -5,6 +5,7 @@ import torch.nn.functional as TF
 from ..engine import grads
 from ..ops.distill import TopLogits, distill_loss, top_logits  # noqa: F401
 from ..ops.functional import _ref
+from ..ops.gated import gated_linear  # noqa: F401
 from ..ops.functional import (  # noqa: F401
     ChannelSlab,
     DenseSlab,

@@ -18,6 +18,7 @@ import torch
 import torch.nn as nn
 
 from ..ops import functional as OF
+from ..ops.gated import gated_linear
 
 _STATS_ATTR = "_pca_stats"
 
@@ -85,6 +86,28 @@ class Linear(nn.Linear):
         if x.dtype != self.weight.dtype:
             x = x.to(self.weight.dtype)
         return nn.functional.linear(x, self.weight, self.bias)
+
+
+class GatedLinear(nn.Module):
+    """act(x Wg^T) * (x Wu^T): the widening half of a gated feed-forward block (a ``Linear`` back to
+    the width follows it). fp32 parameters ``weight_gate`` and ``weight_up`` [hidden_features,
+    in_features], initialised as ``Linear`` does; rows are [..., in_features] or the pixels of an
+    NCHW-shaped feature map, in the type they come in (the weights are rounded to it)."""
+
+    def __init__(self, in_features, hidden_features, act="swish"):
+        super().__init__()
+        self.in_features, self.hidden_features, self.act = in_features, hidden_features, act
+        self.weight_gate = nn.Parameter(torch.empty(hidden_features, in_features))
+        self.weight_up = nn.Parameter(torch.empty(hidden_features, in_features))
+        bound = OF.kaiming_fan_in_bound(in_features)
+        for w in (self.weight_gate, self.weight_up):
+            nn.init.uniform_(w, -bound, bound)
+
+    def forward(self, x):
+        return gated_linear(x, self.weight_gate, self.weight_up, self.act)
+
+    def extra_repr(self):
+        return f"{self.in_features}, {self.hidden_features}, act={self.act!r}"
 
 
 class ReLU(nn.ReLU):
