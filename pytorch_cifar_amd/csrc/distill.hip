@@ -168,103 +168,182 @@ __device__ __forceinline__ int key_index(uint64_t k) {
   return kDistillMaxClasses - 1 - (int)(k & (kDistillMaxClasses - 1));
 }
 
-// Radix selection, 8 bits of the key a pass from the top: exactly k keys have
-// (key & mask) >= prefix when it ends. Right for any row (NaN, all equal, all -inf); the many
-// equal leading bits of a row make its histogram updates collide, so it is the second choice.
+constexpr int kList = 2048;   // candidates that are ranked
+// a selection may end with this many candidates: ranking them costs less than a further pass
+__device__ __forceinline__ int enough(int k) { return k + k / 2 + 64; }
+static_assert(kDistillMaxK + kDistillMaxK / 2 + 64 <= kList, "candidates fit");
+
+// The largest bound of the form lo + (hi - lo) / 2 ... for which at least k keys are as large,
+// halving until at most enough(k) are. Keys differ, so it ends for any row (NaN, all equal, all
+// -inf), after at most 50 passes.
 template <typename T, int BLOCK, int NC>
-__device__ void select_radix(const Row<T, BLOCK, NC>& row, int k, uint32_t* hist, uint64_t* sh,
-                             uint64_t* list) {
-  constexpr int kBits = 32 + kIdxBits;
-  uint64_t prefix = 0, mask = 0;
-  int need = k;
-  for (int top = kBits; top > 0; top -= 8) {
-    const int shift = top > 8 ? top - 8 : 0;
-    const uint32_t digits = (1u << (top - shift)) - 1;
-    for (int i = threadIdx.x; i < 256; i += BLOCK) hist[i] = 0;
-    __syncthreads();
-    row.each([&](int c, const float* f) {
+__device__ uint64_t bound_of_keys(const Row<T, BLOCK, NC>& row, int k, int* red) {
+  uint64_t lo = 0, hi = 1ull << (32 + kIdxBits);
+  int n = row.V;
+  while (n > enough(k)) {
+    const uint64_t mid = lo + (hi - lo) / 2;
+    int c = 0;
+    row.each([&](int ch, const float* f) {
 #pragma unroll
       for (int j = 0; j < kVE<T>; ++j) {
-        const int idx = c * kVE<T> + j;
-        const uint64_t key = order_key(f[j], idx);
-        if (idx < row.V && (key & mask) == prefix)
-          atomicAdd(&hist[(uint32_t)(key >> shift) & digits], 1u);
+        const int idx = ch * kVE<T> + j;
+        c += idx < row.V && order_key(f[j], idx) >= mid;
       }
     });
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int b = (int)digits, above = 0;
-      while (b > 0 && above + (int)hist[b] < need) above += hist[b--];
-      sh[0] = prefix | ((uint64_t)b << shift);
-      sh[1] = (uint64_t)(need - above);
-      sh[2] = hist[b];
-    }
-    __syncthreads();
-    prefix = sh[0];
-    need = (int)sh[1];
-    mask |= (uint64_t)digits << shift;
-    const bool all = (int)sh[2] == need;   // the whole bin is taken: no further bits needed
-    __syncthreads();
-    if (all) break;
+    c = block_fold<BLOCK>(c, red, SumOp());
+    if (c >= k) lo = mid, n = c;
+    else hi = mid;
   }
-  if (threadIdx.x == 0) hist[0] = 0;
-  __syncthreads();
-  row.each([&](int c, const float* f) {
-#pragma unroll
-    for (int j = 0; j < kVE<T>; ++j) {
-      const int idx = c * kVE<T> + j;
-      const uint64_t key = order_key(f[j], idx);
-      if (idx < row.V && (key & mask) >= prefix) {
-        const uint32_t at = atomicAdd(&hist[0], 1u);
-        if (at < (uint32_t)k) list[at] = key;
-      }
-    }
-  });
-  __syncthreads();
+  return lo;
 }
 
+// The same over the maxima of the row's threads (one wave, BLOCK / 64 of them a lane): at least k
+// logits are as large as the k-th largest of them, and in a row in no particular order few more.
+template <int BLOCK>
+__device__ uint32_t bound_of_maxima(const uint32_t* maxima, int k) {
+  constexpr int N = BLOCK / 64;
+  uint32_t v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = maxima[threadIdx.x + i * 64];
+  uint64_t lo = 0, hi = 1ull << 32;
+  int n = BLOCK;
+  while (n > k + k / 4 + 8 && hi - lo > 1) {
+    const uint32_t mid = (uint32_t)(lo + (hi - lo) / 2);
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) c += __popcll(__ballot(v[i] >= mid));
+    if (c >= k) lo = mid, n = c;
+    else hi = mid;
+  }
+  return (uint32_t)lo;
+}
+
+// One pass over the row gives each thread its maximum and its sum of exponentials (relative to its
+// running maximum). The k largest are then sought among the logits of the threads whose maximum
+// reaches a bound; a row that defeats the bound (NaN, many equal logits, k near the number of
+// threads) is halved by counting.
 template <typename T, int BLOCK, int NC>
 __global__ __launch_bounds__(BLOCK) void top_logits_kernel(const T* __restrict__ z, int64_t ld,
-                                                           int V, int k, float c,
-                                                           double inv_t,
+                                                           int V, int k, float c, double inv_t,
                                                            T* __restrict__ values,
                                                            int32_t* __restrict__ indices,
                                                            float* __restrict__ lse) {
   __shared__ double red[16];
-  __shared__ uint32_t hist[256];
-  __shared__ uint64_t sh[4];
-  __shared__ uint64_t list[kDistillMaxK];
+  __shared__ uint32_t maxima[BLOCK];
+  __shared__ uint64_t list[kList];
+  __shared__ uint32_t found, bound;
   const int64_t r = blockIdx.x;
   Row<T, BLOCK, NC> row;
   row.load(z + r * ld, V);
 
-  float m = -INFINITY;
+  float m = -INFINITY, base = 0.f, s = 0.f;   // base: m where it is finite
   row.each([&](int, const float* f) {
+    float cm = f[0];
 #pragma unroll
-    for (int j = 0; j < kVE<T>; ++j) m = fmaxf(m, f[j]);
-  });
-  m = block_fold<BLOCK>(m, reinterpret_cast<float*>(red), MaxOp());
-  if (isinf(m)) m = 0.f;   // a row of -inf: log 0; one with +inf: log inf
-  float s = 0.f;
-  row.each([&](int, const float* f) {
+    for (int j = 1; j < kVE<T>; ++j) cm = fmaxf(cm, f[j]);
+    m = fmaxf(m, cm);
+    const float b = isinf(m) ? 0.f : m;
+    s *= __builtin_amdgcn_exp2f((base - b) * c);
+    base = b;
 #pragma unroll
-    for (int j = 0; j < kVE<T>; ++j) s += __builtin_amdgcn_exp2f((f[j] - m) * c);
+    for (int j = 0; j < kVE<T>; ++j) s += __builtin_amdgcn_exp2f((f[j] - b) * c);
   });
+  // (a row of -inf: log 0; one with +inf: log inf; NaN stays)
+  float all = block_fold<BLOCK>(m, reinterpret_cast<float*>(red), MaxOp());
+  if (isinf(all)) all = 0.f;
+  s *= __builtin_amdgcn_exp2f((base - all) * c);
   const double sum = block_fold<BLOCK>((double)s, red, SumOp());
-  if (threadIdx.x == 0) lse[r] = (float)((double)m * inv_t + log(sum));
+  if (threadIdx.x == 0) {
+    lse[r] = (float)((double)all * inv_t + log(sum));
+    found = 0;
+    bound = 0;
+  }
+  const uint32_t mine = order_bits(m);
+  maxima[threadIdx.x] = mine;
+  __syncthreads();
 
-  Row<T, BLOCK, 0> again;
-  again.load(row.p, V);
-  select_radix(again, k, hist, sh, list);
-  // the place of each kept logit is the number of kept ones before it
-  for (int i = threadIdx.x; i < k; i += BLOCK) {
+  bool few = k <= BLOCK / 4 * 3 && sum == sum;   // (a thread's maximum passes over NaN)
+  if (few) {
+    if (threadIdx.x < 64) {
+      const uint32_t b = bound_of_maxima<BLOCK>(maxima, k);
+      if (threadIdx.x == 0) bound = b;
+    }
+    __syncthreads();
+    const uint32_t b = bound;
+    if (mine >= b) {
+      row.each([&](int ch, const float* f) {
+#pragma unroll
+        for (int j = 0; j < kVE<T>; ++j) {
+          const int idx = ch * kVE<T> + j;
+          if (idx < V && order_bits(f[j]) >= b) {
+            const uint32_t at = atomicAdd(&found, 1u);
+            if (at < kList) list[at] = order_key(f[j], idx);
+          }
+        }
+      });
+    }
+    __syncthreads();
+    few = found <= kList;
+  }
+  if (!few) {
+    __syncthreads();
+    if (threadIdx.x == 0) found = 0;
+    const uint64_t b = bound_of_keys(row, k, reinterpret_cast<int*>(red));
+    __syncthreads();
+    row.each([&](int ch, const float* f) {
+#pragma unroll
+      for (int j = 0; j < kVE<T>; ++j) {
+        const int idx = ch * kVE<T> + j;
+        const uint64_t key = order_key(f[j], idx);
+        if (idx < V && key >= b) {
+          const uint32_t at = atomicAdd(&found, 1u);
+          if (at < kList) list[at] = key;
+        }
+      }
+    });
+    __syncthreads();
+  }
+  // a candidate's place is the number of candidates before it
+  const int n = (int)found;
+  for (int i = threadIdx.x; i < n; i += BLOCK) {
     const uint64_t key = list[i];
     int at = 0;
-    for (int j = 0; j < k; ++j) at += list[j] > key;
-    const int idx = key_index(key);
-    values[r * k + at] = row.p[idx];
-    indices[r * k + at] = idx;
+    for (int j = 0; j < n; ++j) at += list[j] > key;
+    if (at < k) {
+      const int idx = key_index(key);
+      values[r * k + at] = row.p[idx];
+      indices[r * k + at] = idx;
+    }
   }
+}
+
+// Rows of up to 64 classes: a wave each, a class a lane. The place of a logit is the number of
+// logits before it, counted over the lanes.
+template <typename T>
+__global__ __launch_bounds__(256) void top_small_kernel(const T* __restrict__ z, int64_t ld,
+                                                        int64_t R, int V, int k, float c,
+                                                        double inv_t, T* __restrict__ values,
+                                                        int32_t* __restrict__ indices,
+                                                        float* __restrict__ lse) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = blockIdx.x * 4ll + (threadIdx.x >> 6);
+  if (r >= R) return;
+  const T v = z[r * ld + min(lane, V - 1)];
+  const float f = lane < V ? to_f(v) : -INFINITY;
+  float m = wave_max(f);
+  if (isinf(m)) m = 0.f;
+  const float s = wave_sum(__builtin_amdgcn_exp2f((f - m) * c));
+  const uint32_t key = order_bits(f);
+  int at = 0;
+  for (int j = 0; j < V; ++j) {
+    const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)key, j);
+    at += other > key || (other == key && j < lane);
+  }
+  if (lane < V && at < k) {
+    values[r * k + at] = v;
+    indices[r * k + at] = lane;
+  }
+  if (lane == 0) lse[r] = (float)((double)m * inv_t + log((double)s));
 }
 
 // ------------------------------------------------------------------------------ distill_loss
@@ -516,15 +595,16 @@ __global__ __launch_bounds__(256) void scale_rows_kernel(T* __restrict__ dz, int
   }
 }
 
-// Threads and register chunks of a row: calls fn<BLOCK, NC>.
+// Threads and register chunks of a row: calls fn<BLOCK, NC>. again: long rows are read again
 template <typename T, typename F>
-void pick_row(int V, F&& fn) {
+void pick_row(int V, bool again, F&& fn) {
   using std::integral_constant;
   const int n = (V + kVE<T> - 1) / kVE<T>;
   if (n <= 64) fn(integral_constant<int, 64>(), integral_constant<int, 1>());
   else if (n <= 256) fn(integral_constant<int, 64>(), integral_constant<int, 4>());
   else if (n <= 1024) fn(integral_constant<int, 256>(), integral_constant<int, 4>());
   else if (n <= 2048) fn(integral_constant<int, 256>(), integral_constant<int, 8>());
+  else if (again) fn(integral_constant<int, 1024>(), integral_constant<int, 0>());
   else if (n <= 8192) fn(integral_constant<int, 1024>(), integral_constant<int, 8>());
   else if (n <= 16384) fn(integral_constant<int, 1024>(), integral_constant<int, 16>());
   else fn(integral_constant<int, 1024>(), integral_constant<int, 0>());
@@ -544,7 +624,13 @@ void top_logits_launch(const void* z, int type, int64_t ld, int64_t R, int V, in
   const float c = (float)(1.4426950408889634 / temp);
   pick_type(type, [&](auto tv) {
     using T = decltype(tv);
-    pick_row<T>(V, [&](auto block, auto nc) {
+    if (V <= 64) {
+      hipLaunchKernelGGL((top_small_kernel<T>), dim3((uint32_t)((R + 3) / 4)), dim3(256), 0, st,
+                         reinterpret_cast<const T*>(z), ld, R, V, k, c, 1.0 / temp,
+                         reinterpret_cast<T*>(values), indices, lse);
+      return;
+    }
+    pick_row<T>(V, true, [&](auto block, auto nc) {
       constexpr int BLOCK = decltype(block)::value, NC = decltype(nc)::value;
       hipLaunchKernelGGL((top_logits_kernel<T, BLOCK, NC>), dim3((uint32_t)R), dim3(BLOCK), 0, st,
                          reinterpret_cast<const T*>(z), ld, V, k, c, 1.0 / temp,
@@ -558,7 +644,7 @@ void distill_launch(const DistillArgs& a, hipStream_t st) {
   const size_t lds = (size_t)a.K * 12 + (size_t)((a.V + 31) / 32) * 4;
   pick_type(a.type, [&](auto tv) {
     using T = decltype(tv);
-    pick_row<T>(a.V, [&](auto block, auto nc) {
+    pick_row<T>(a.V, false, [&](auto block, auto nc) {
       constexpr int BLOCK = decltype(block)::value, NC = decltype(nc)::value;
       if (a.dz)
         hipLaunchKernelGGL((distill_kernel<T, BLOCK, NC, true>), dim3((uint32_t)a.R), dim3(BLOCK),
