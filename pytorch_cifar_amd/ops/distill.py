@@ -13,12 +13,13 @@ from typing import NamedTuple
 import torch
 import torch.nn.functional as F
 
-from .functional import _C, _is_unit, _ref
+from .. import _native
+from .functional import _C, _ref
 
 MAX_CLASSES = 1 << 18
 MAX_K = 1024
 REST = 2.0 ** -20        # csrc/distill.h kDistillRest
-_REDUCTION = {"none": 0, "mean": 1, "sum": 2}
+_REDUCTION = ("none", "mean", "sum")
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
@@ -47,12 +48,16 @@ def _check_temperature(t):
     return t
 
 
-def _rows(x):
-    """[..., n] as [rows, n] whose rows are contiguous in themselves (their stride may be any)."""
-    r = x.reshape(-1, x.shape[-1])
-    if (r.shape[1] > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < 0):
-        r = r.contiguous()
-    return r
+def _name_bad_class(logits, indices, target, ignore_index):
+    """Debug mode: name a class outside the row on the host (the kernel NaN-poisons its row)."""
+    n = logits.shape[-1]
+    bad = [("index", indices, indices >= n)]
+    if target is not None:
+        bad.append(("target", target, (target != ignore_index) & ((target < 0) | (target >= n))))
+    for name, x, b in bad:
+        if bool(b.any()):
+            at = b.nonzero()[0].tolist()
+            raise IndexError(f"distill_loss: {name} {int(x[tuple(at)])} at {at} is outside [0, {n})")
 
 
 def top_logits(logits, k, temperature=1.0):
@@ -62,21 +67,19 @@ def top_logits(logits, k, temperature=1.0):
     ``lse`` is taken at ``temperature``, that of the loss that will use it; the values are the
     logits as they are. Not differentiable: a teacher's answer is data to its student.
     """
+    if not _ref(logits):
+        return TopLogits(*_C().top_logits(logits, k, temperature))
     _check_logits(logits)
     t = _check_temperature(temperature)
     n = logits.shape[-1]
     k = int(k)
     if not 1 <= k <= min(n, MAX_K):
         raise ValueError(f"k must be 1 to {min(n, MAX_K)}, got {k}")
-    lead = logits.shape[:-1]
     with torch.no_grad():
-        if _ref(logits):
-            z = logits.float()
-            values, indices = torch.sort(z, dim=-1, descending=True, stable=True)
-            lse = torch.logsumexp(z.double() / t, -1).float()
-            return TopLogits(values[..., :k].to(logits.dtype), indices[..., :k].to(torch.int32), lse)
-        values, indices, lse = _C().top_logits(_rows(logits.detach()), k, t)
-    return TopLogits(values.view(*lead, k), indices.view(*lead, k), lse.view(lead))
+        z = logits.float()
+        values, indices = torch.sort(z, dim=-1, descending=True, stable=True)
+        lse = torch.logsumexp(z.double() / t, -1).float()
+        return TopLogits(values[..., :k].to(logits.dtype), indices[..., :k].to(torch.int32), lse)
 
 
 def _ref_distill(z, values, indices, lse, target, t, alpha, tail, ignore_index):
@@ -125,31 +128,6 @@ def _ref_distill(z, values, indices, lse, target, t, alpha, tail, ignore_index):
     return loss * torch.where(bad, math.nan, 1.0).to(loss)
 
 
-class _Distill(torch.autograd.Function):
-    """The forward pass computes the gradient for a unit seed from the row it holds in registers
-    and hands it to the backward, which scales it where the seed is not one. A second backward of
-    a retained graph computes it again from the saved logits."""
-
-    @staticmethod
-    def forward(ctx, z, values, indices, lse, target, cfg):
-        loss, dz = _C().distill(z, values, indices, lse, target, *cfg, True)
-        ctx.save_for_backward(z, values, indices, lse, target)
-        ctx.cfg = cfg
-        ctx.dz = dz
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dloss):
-        saved = ctx.saved_tensors
-        dz, ctx.dz = ctx.dz, None
-        if dz is None:
-            _, dz = _C().distill(*saved, *ctx.cfg, True)
-        if not _is_unit(dloss):
-            _C().scale_rows_(dz, dloss.float().reshape(-1).contiguous())
-        return dz, None, None, None, None, None
-
-
 def distill_loss(logits, top, target=None, temperature=1.0, alpha=None, tail=False,
                  reduction="mean", ignore_index=-100):
     """Loss of a student's ``logits`` [..., classes] against a teacher's ``top`` logits.
@@ -171,20 +149,25 @@ def distill_loss(logits, top, target=None, temperature=1.0, alpha=None, tail=Fal
 
     Teacher's side is data: gradients flow to ``logits`` alone.
     """
-    _check_logits(logits)
-    t = _check_temperature(temperature)
-    if reduction not in _REDUCTION:
-        raise ValueError(f"reduction must be one of {sorted(_REDUCTION)}, got {reduction!r}")
     if alpha is None:
         if target is not None:
             raise ValueError("alpha (the weight of the teacher's term) must be given with a target")
         alpha = 1.0
+    values, indices, lse = top if len(top) == 3 else (*top, None)
+    if not _ref(logits):
+        if _native._debug:
+            _name_bad_class(logits, indices, target if alpha != 1 else None, ignore_index)
+        return _C().distill_loss(logits, values, indices, lse, target, temperature, alpha, tail,
+                                 reduction, ignore_index, _native._debug)
+    _check_logits(logits)
+    t = _check_temperature(temperature)
+    if reduction not in _REDUCTION:
+        raise ValueError(f"reduction must be one of {_REDUCTION}, got {reduction!r}")
     alpha = float(alpha)
     if not 0 <= alpha <= 1:
         raise ValueError(f"alpha must be in [0, 1], got {alpha}")
     if target is None and alpha != 1:
         raise ValueError("alpha below 1 needs a target")
-    values, indices, lse = top if len(top) == 3 else (*top, None)
     lead = logits.shape[:-1]
     k = values.shape[-1] if values.dim() else 0
     if values.shape[:-1] != lead or indices.shape != values.shape or values.dim() < 1:
@@ -208,32 +191,10 @@ def distill_loss(logits, top, target=None, temperature=1.0, alpha=None, tail=Fal
         if x is not None and x.requires_grad:
             raise ValueError(f"{name} requires grad: a teacher's answer is data, detach it")
 
-    z = _rows(logits)
-    values, indices = values.reshape(-1, k), indices.reshape(-1, k)
-    lse = lse.reshape(-1) if tail else None
-    target = target.reshape(-1) if target is not None else None
-    if _ref(logits):
-        rows = _ref_distill(z, values, indices, lse, target, t, alpha, tail, ignore_index)
-        loss = rows if reduction == "none" else rows.mean() if reduction == "mean" else rows.sum()
-        loss = loss.float()
-    else:
-        from .. import _native
-
-        if _native._debug:   # name a bad class on the host (the kernel NaN-poisons its row)
-            for name, x, low in (("index", indices, None), ("target", target, ignore_index)):
-                if x is None or (name == "target" and alpha == 1):
-                    continue
-                bad = x >= z.shape[1] if low is None else ((x != low) & ((x < 0) | (x >= z.shape[1])))
-                if bool(bad.any()):
-                    at = bad.nonzero()[0].tolist()
-                    raise IndexError(f"distill_loss: {name} {int(x[tuple(at)])} at {at} is outside "
-                                     f"[0, {z.shape[1]})")
-        args = (z, values.contiguous(), indices.contiguous(),
-                lse.contiguous() if tail else None,
-                target.contiguous() if target is not None else None)
-        cfg = (t, alpha, bool(tail), _REDUCTION[reduction], int(ignore_index))
-        if torch.is_grad_enabled() and logits.requires_grad:
-            loss = _Distill.apply(*args, cfg)
-        else:
-            loss, _ = _C().distill(*args, *cfg, False)
-    return loss.view(lead) if reduction == "none" else loss
+    rows = _ref_distill(logits.reshape(-1, logits.shape[-1]), values.reshape(-1, k),
+                        indices.reshape(-1, k), lse.reshape(-1) if tail else None,
+                        target.reshape(-1) if target is not None else None, t, alpha, tail,
+                        ignore_index)
+    if reduction == "none":
+        return rows.float().view(lead)
+    return (rows.mean() if reduction == "mean" else rows.sum()).float()

@@ -2378,6 +2378,8 @@ def unit_grad(loss: torch.Tensor) -> torch.Tensor:
     if t is None:
         t = torch.ones(loss.shape, dtype=loss.dtype, device=loss.device)
         _UNIT[key] = t
+        if t.is_cuda:
+            _C().register_unit_seed(t)
     return t
 
 

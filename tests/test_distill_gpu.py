@@ -390,12 +390,62 @@ def test_refusals_on_the_gpu():
         PF.top_logits(z.cuda(), 51)
     from pytorch_cifar_amd import _native
 
-    C = _native.lib()
-    with pytest.raises(RuntimeError):
-        C.top_logits(z.cuda().t(), 1, 1.0)                   # classes not contiguous
-    with pytest.raises(RuntimeError):
-        C.top_logits(z, 1, 1.0)
-    with pytest.raises(RuntimeError):
-        C.distill(z.cuda(), g.values[:, ::2], g.indices[:, ::2], None, None, 1.0, 1.0, False, 1, -100, True)
-    with pytest.raises(RuntimeError):
-        C.distill(z.cuda(), g.values, g.indices, None, None, 1.0, 1.0, True, 1, -100, True)
+    with pytest.raises(ValueError):
+        _native.lib().top_logits(z, 1, 1.0)
+
+
+def test_second_derivatives_are_refused():
+    z, top, y = distill_inputs(4, 50, 3, torch.float32, 1.0)
+    x = z.cuda().requires_grad_(True)
+    (g,) = torch.autograd.grad(PF.distill_loss(x, gpu_top(top)), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        g.sum().backward()
+
+
+def test_changed_logits_are_noticed():
+    z, top, y = distill_inputs(4, 50, 3, torch.float32, 1.0)
+    x = z.cuda().requires_grad_(True)
+    w = x * 1.0
+    loss = PF.distill_loss(w, gpu_top(top))
+    w.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified"):
+        loss.backward()
+
+
+@pytest.mark.parametrize("kw, err", [
+    (dict(temperature=0.0), ValueError), (dict(temperature=math.inf), ValueError),
+    (dict(alpha=1.5), ValueError), (dict(alpha=0.5), ValueError), (dict(reduction="max"), ValueError),
+    (dict(target=torch.zeros(4, dtype=torch.int64)), ValueError),
+    (dict(target=torch.zeros(4, dtype=torch.int32), alpha=0.5), ValueError),
+    (dict(target=torch.zeros(3, dtype=torch.int64), alpha=0.5), ValueError),
+])
+def test_argument_refusals(kw, err):
+    z, top, _ = distill_inputs(4, 50, 3, torch.float32, 1.0)
+    kw = {k: v.cuda() if torch.is_tensor(v) else v for k, v in kw.items()}
+    with pytest.raises(err):
+        PF.distill_loss(z.cuda(), gpu_top(top), **kw)
+
+
+def test_refuses_what_does_not_fit():
+    z, top, _ = distill_inputs(7, 50, 5, torch.float32, 1.0)
+    z, top, T = z.cuda(), gpu_top(top), PF.TopLogits
+    for err, args, kw in [
+            (ValueError, (z, T(top.values, top.indices, None)), dict(tail=True)),
+            (ValueError, (z, T(top.values, top.indices, top.lse[:3])), dict(tail=True)),
+            (ValueError, (z, T(top.values, top.indices, top.lse.double())), dict(tail=True)),
+            (ValueError, (z[:3], top), {}),
+            (ValueError, (z, T(top.values[:, :2], top.indices, None)), {}),
+            (TypeError, (z, T(top.values.double(), top.indices, None)), {}),
+            (TypeError, (z, T(top.values, top.indices.short(), None)), {}),
+            (TypeError, (z.double(), top), {}),
+            (ValueError, (z, T(top.values.clone().requires_grad_(True), top.indices, None)), {}),
+            (ValueError, (torch.zeros(7, 0, device="cuda"), top), {})]:
+        with pytest.raises(err):
+            PF.distill_loss(*args, **kw)
+    for err, args, kw in [
+            (ValueError, (z, 51), {}), (ValueError, (z, 0), {}), (ValueError, (z, 1), dict(temperature=-1.0)),
+            (TypeError, (z.int(), 1), {}), (ValueError, (torch.zeros(1, 2000, device="cuda"), 1025), {}),
+            (ValueError, (torch.zeros((), device="cuda"), 1), {}),
+            (ValueError, (torch.zeros(1, (1 << 18) + 1, device="cuda"), 1), {})]:
+        with pytest.raises(err):
+            PF.top_logits(*args, **kw)

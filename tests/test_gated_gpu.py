@@ -307,25 +307,24 @@ def test_changed_weights_are_noticed():
         h.backward(dh)
 
 
+def test_second_derivatives_are_refused():
+    x, wg, wu, dh = inputs(8, 16, 24, torch.bfloat16, 12)
+    x.requires_grad_(True)
+    (g,) = torch.autograd.grad(PF.gated_linear(x, wg, wu), x, dh, create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        g.float().sum().backward()
+
+
 def test_refusals_on_the_gpu():
     x, wg, wu, dh = inputs(8, 16, 24, torch.bfloat16, 12)
-    with pytest.raises(ValueError):
-        PF.gated_linear(x, wg.cpu(), wu)
-    with pytest.raises(TypeError):
-        PF.gated_linear(x, wg.half(), wu.half())
-    from pytorch_cifar_amd import _native
-
-    C = _native.lib()
-    with pytest.raises(RuntimeError):
-        C.gated_fwd(x[:, 1:], wg[:, 1:], wu[:, 1:], 2, False)      # not an operand
-    with pytest.raises(RuntimeError):
-        C.gated_fwd(x, wg, wu[:16], 2, False)
-    with pytest.raises(RuntimeError):
-        C.gated_fwd(x, wg, wu, 4, False)
-    h, g, u = C.gated_fwd(x, wg, wu, 2, True)
-    with pytest.raises(RuntimeError):
-        C.gated_bwd(dh, x, wg, wu, g[:4], u, 16, 2, True, True, False)
-    with pytest.raises(RuntimeError):
-        C.gated_bwd(dh.float(), x, wg, wu, g, u, 16, 2, True, True, False)
-    with pytest.raises(RuntimeError):
-        C.gated_bwd(dh, x, wg, wu, g, u, 4, 2, True, True, False)
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device="cuda")   # noqa: E731
+    for err, args in [
+            (ValueError, (x, wg.cpu(), wu)), (TypeError, (x, wg.half(), wu.half())),
+            (TypeError, (x, wg.float(), wu)), (ValueError, (x[:, :8], wg, wu)),
+            (ValueError, (x, wg, wu[:16])), (ValueError, (x, wg[0], wu[0])),
+            (ValueError, (x, wg, wu, "gelu")), (TypeError, (x.long(), wg, wu)),
+            (TypeError, (x.double(), wg.double(), wu.double())), (ValueError, (x, wg[:0], wu[:0])),
+            (ValueError, (z(2, 0), z(4, 0), z(4, 0))), (ValueError, (z(1, 16)[0, 0], wg, wu)),
+            (ValueError, (z(1, (1 << 19) + 8), z(1, (1 << 19) + 8), z(1, (1 << 19) + 8)))]:
+        with pytest.raises(err):
+            PF.gated_linear(*args)
