@@ -2,9 +2,8 @@
 // log-sum-exp (top_logits), and the loss of a student's logits against them with its gradient
 // (distill_*). Rows are [R][V] in fp32 / bf16 / fp16 with any row stride; one workgroup a row.
 //
-// Both read each logit once: a row of up to 16 chunks of 16 bytes a thread stays in registers
-// between its passes (maximum, then sum of exponentials, then gradient or selection); longer rows
-// are read again for each pass.
+// Rows of up to 1024 chunks of 16 bytes stay in registers between their passes; longer ones are
+// streamed in one pass (sums, selection), which the gradient follows with a second one.
 #include "distill.h"
 
 #include <algorithm>
@@ -51,7 +50,7 @@ __device__ __forceinline__ uint4 pack(const float* f, f16) {
 template <typename T>
 __device__ __forceinline__ uint4 load_chunk(const T* __restrict__ row, int c, int V) {
   uint4 u;
-  const T* p = row + (size_t)c * kVE<T>;
+  const T* p = row + (uint32_t)c * kVE<T>;
   if ((c + 1) * kVE<T> <= V) {
     __builtin_memcpy(&u, p, 16);
     return u;
@@ -62,12 +61,19 @@ __device__ __forceinline__ uint4 load_chunk(const T* __restrict__ row, int c, in
   return pack(f, T());
 }
 
-template <typename T>
-__device__ __forceinline__ void store_chunk(T* __restrict__ row, int c, int V, const float* f) {
+// (STREAM: past the caches, which then keep the rows that are read again: distill_loss with gradient,
+// 4096 x 128000 bf16, 514 -> 478 us)
+template <bool STREAM = false, typename T>
+__device__ __forceinline__ void store_chunk(T* __restrict__ row, int c, int V, const float* f,
+                                            bool whole = false) {
   const uint4 u = pack(f, T());
-  T* p = row + (size_t)c * kVE<T>;
-  if ((c + 1) * kVE<T> <= V) {
-    __builtin_memcpy(p, &u, 16);
+  T* p = row + (uint32_t)c * kVE<T>;
+  if (whole || (c + 1) * kVE<T> <= V) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(2)));
+    if constexpr (STREAM)
+      __builtin_nontemporal_store((u32x4){u.x, u.y, u.z, u.w}, reinterpret_cast<u32x4*>(p));
+    else
+      __builtin_memcpy(p, &u, 16);
     return;
   }
   T h[kVE<T>];
@@ -95,9 +101,12 @@ struct Row {
       }
     }
   }
-  // fn(chunk number, its elements as float)
+  // fn(chunk number, its elements as float, whether it is known to be whole)
   template <typename F>
   __device__ __forceinline__ void each(F&& fn) const {
+    constexpr std::integral_constant<bool, true> whole;
+    constexpr std::integral_constant<bool, false> any;
+    float f[kVE<T>];
     if constexpr (NC > 0) {
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
@@ -106,22 +115,50 @@ struct Row {
           // (opaque, so that the passes unpack anew: kept across them, the floats spill)
           uint4 v = u[i];
           asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w));
-          float f[kVE<T>];
           unpack(v, f, T());
-          fn(c, f);
+          fn(c, f, any);
         }
       }
     } else {
-#pragma unroll 4
-      for (int c = threadIdx.x; c < n; c += BLOCK) {
-        const uint4 v = load_chunk(p, c, V);
-        float f[kVE<T>];
-        unpack(v, f, T());
-        fn(c, f);
+      // (the next two chunks are on their way while two are worked on; without the barrier the
+      // compiler waits for each load where it is issued)
+      constexpr int U = 2;
+      const int rounds = V / kVE<T> / BLOCK / U;
+      int c = threadIdx.x;
+      uint4 v[U], next[U];
+      auto fetch = [&](uint4* to, int at) {
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+          __builtin_memcpy(&to[j], p + (uint32_t)(at + j * BLOCK) * kVE<T>, 16);
+      };
+      if (rounds > 0) fetch(v, c);
+      for (int i = 0; i < rounds; ++i, c += U * BLOCK) {
+        if (i + 1 < rounds) fetch(next, c + U * BLOCK);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+          unpack(v[j], f, T());
+          fn(c + j * BLOCK, f, whole);
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) v[j] = next[j];
+      }
+      for (; c < n; c += BLOCK) {
+        unpack(load_chunk(p, c, V), f, T());
+        fn(c, f, any);
       }
     }
   }
 };
+
+// the largest of a chunk (a NaN is passed over) and m
+template <int N>
+__device__ __forceinline__ float chunk_max(const float* f, float m) {
+#pragma unroll
+  for (int j = 0; j < N; j += 2)
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(m), "v"(f[j]), "v"(f[j + 1]));
+  return m;
+}
 
 struct MaxOp {
   template <typename A>
@@ -134,11 +171,18 @@ struct SumOp {
   __device__ __forceinline__ A operator()(A a, A b) const { return a + b; }
 };
 
+// v of N neighbouring lanes, in a fixed order
+template <int N = 64, typename A, typename Op>
+__device__ __forceinline__ A wave_fold(A v, Op op) {
+#pragma unroll
+  for (int o = N / 2; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
 // v of all threads, folded in a fixed order; every thread gets the result. red: BLOCK/64 values.
 template <int BLOCK, typename A, typename Op>
 __device__ __forceinline__ A block_fold(A v, A* red, Op op) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
+  v = wave_fold(v, op);
   if constexpr (BLOCK == 64) return v;
   constexpr int NW = BLOCK / 64;
   __syncthreads();   // (red may still be read by the fold before)
@@ -148,6 +192,29 @@ __device__ __forceinline__ A block_fold(A v, A* red, Op op) {
 #pragma unroll
   for (int w = 1; w < NW; ++w) r = op(r, red[w]);
   return r;
+}
+
+// Sum of 2^(x - base) over a thread's x = z c, in one pass without the maximum: a term costs one
+// multiply-add, the exponential and the add. The base is the first chunk's largest x, as a whole
+// number (sums of different bases are joined by exact powers of two): 2^60 above and all below it
+// is room for what follows. A row that leaves it (a first chunk of masked classes, |x| past 2^22,
+// infinities, NaN) is summed again against its maximum (`plain` below).
+constexpr float kNoBase = -4194304.f, kFar = 4194304.f;
+constexpr double kMost = 1152921504606846976.0;   // 2^60
+
+template <int N>
+__device__ __forceinline__ void first_base(float& base, const float* f, float c) {
+  if (base != kNoBase) return;
+  const float x = chunk_max<N>(f, f[0]) * c;
+  if (x > kNoBase && x < kFar) base = rintf(x);
+}
+
+__device__ __forceinline__ float term(float z, float c, float base) {
+  return __builtin_amdgcn_exp2f(fmaf(z, c, -base));
+}
+// the same against a maximum m that may be anything
+__device__ __forceinline__ float term_at(float z, float m, float c) {
+  return __builtin_amdgcn_exp2f((z - m) * c);
 }
 
 // ------------------------------------------------------------------------------- top_logits
@@ -161,6 +228,9 @@ __device__ __forceinline__ uint32_t order_bits(float f) {
   const uint32_t b = __float_as_uint(f + 0.f);   // (-0 + 0 is +0)
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float float_of(uint32_t bits) {   // of order_bits
+  return __uint_as_float(bits & 0x80000000u ? bits ^ 0x80000000u : ~bits);
+}
 __device__ __forceinline__ uint64_t order_key(float f, int idx) {
   return ((uint64_t)order_bits(f) << kIdxBits) | (uint32_t)(kDistillMaxClasses - 1 - idx);
 }
@@ -168,7 +238,7 @@ __device__ __forceinline__ int key_index(uint64_t k) {
   return kDistillMaxClasses - 1 - (int)(k & (kDistillMaxClasses - 1));
 }
 
-constexpr int kList = 2048;   // candidates that are ranked
+constexpr int kList = 2048;   // candidates that are ranked at most
 // a selection may end with this many candidates: ranking them costs less than a further pass
 __device__ __forceinline__ int enough(int k) { return k + k / 2 + 64; }
 static_assert(kDistillMaxK + kDistillMaxK / 2 + 64 <= kList, "candidates fit");
@@ -183,7 +253,7 @@ __device__ uint64_t bound_of_keys(const Row<T, BLOCK, NC>& row, int k, int* red)
   while (n > enough(k)) {
     const uint64_t mid = lo + (hi - lo) / 2;
     int c = 0;
-    row.each([&](int ch, const float* f) {
+    row.each([&](int ch, const float* f, auto) {
 #pragma unroll
       for (int j = 0; j < kVE<T>; ++j) {
         const int idx = ch * kVE<T> + j;
@@ -200,14 +270,22 @@ __device__ uint64_t bound_of_keys(const Row<T, BLOCK, NC>& row, int k, int* red)
 // The same over the maxima of the row's threads (one wave, BLOCK / 64 of them a lane): at least k
 // logits are as large as the k-th largest of them, and in a row in no particular order few more.
 template <int BLOCK>
-__device__ uint32_t bound_of_maxima(const uint32_t* maxima, int k) {
+__device__ uint32_t bound_of_maxima(const uint32_t* maxima, int k, int spare) {   // at most k + spare maxima reach it, if they differ
   constexpr int N = BLOCK / 64;
   uint32_t v[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = maxima[threadIdx.x + i * 64];
-  uint64_t lo = 0, hi = 1ull << 32;
+  uint32_t least = v[0], most = v[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) least = min(least, v[i]), most = max(most, v[i]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    least = min(least, (uint32_t)__shfl_xor((int)least, o, 64));
+    most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
+  }
+  uint64_t lo = least, hi = most + 1ull;
   int n = BLOCK;
-  while (n > k + k / 4 + 8 && hi - lo > 1) {
+  while (n > k + spare && hi - lo > 1) {
     const uint32_t mid = (uint32_t)(lo + (hi - lo) / 2);
     int c = 0;
 #pragma unroll
@@ -218,79 +296,170 @@ __device__ uint32_t bound_of_maxima(const uint32_t* maxima, int k) {
   return (uint32_t)lo;
 }
 
-// One pass over the row gives each thread its maximum and its sum of exponentials (relative to its
-// running maximum). The k largest are then sought among the logits of the threads whose maximum
-// reaches a bound; a row that defeats the bound (NaN, many equal logits, k near the number of
-// threads) is halved by counting.
+// One pass over the row gives each thread its maximum, its sum of exponentials, and, where the row is
+// long, the candidates: a bound on the first four chunks of the threads, low enough that with some
+// three standard deviations to spare k logits of a row in random order reach it, is known after them,
+// and what reaches it is put on a list as it comes by. A row whose list is short or overflows (one
+// in some other order) takes the chunks of the threads whose maximum reaches a bound on all maxima; a
+// row that defeats this too (NaN, many equal logits, k near the number of threads) is halved by
+// counting.
+//
+// Bound by the read: 2048 x 128000 bf16, k 64, in 102 us (5.1 TB/s; a large copy reaches 4.85).
 template <typename T, int BLOCK, int NC>
-__global__ __launch_bounds__(BLOCK) void top_logits_kernel(const T* __restrict__ z, int64_t ld,
-                                                           int V, int k, float c, double inv_t,
-                                                           T* __restrict__ values,
-                                                           int32_t* __restrict__ indices,
-                                                           float* __restrict__ lse) {
+__global__ __launch_bounds__(BLOCK)
+__attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void top_logits_kernel(
+    const T* __restrict__ z, int64_t ld, int V, int k, float c, double inv_t,
+    T* __restrict__ values, int32_t* __restrict__ indices, float* __restrict__ lse) {
   __shared__ double red[16];
+  constexpr int NW = BLOCK / 64, VE = kVE<T>;
+  __shared__ struct { float m, base, s; } part[NW];
   __shared__ uint32_t maxima[BLOCK];
+  __shared__ uint16_t who[BLOCK];
   __shared__ uint64_t list[kList];
-  __shared__ uint32_t found, bound;
+  __shared__ uint32_t found, who_n, bound;
   const int64_t r = blockIdx.x;
   Row<T, BLOCK, NC> row;
   row.load(z + r * ld, V);
 
-  float m = -INFINITY, base = 0.f, s = 0.f;   // base: m where it is finite
-  row.each([&](int, const float* f) {
-    float cm = f[0];
-#pragma unroll
-    for (int j = 1; j < kVE<T>; ++j) cm = fmaxf(cm, f[j]);
+  float m = -INFINITY, base = kNoBase, s = 0.f;
+  auto take = [&](const float* f) {
+    const float cm = chunk_max<VE>(f, -INFINITY);
     m = fmaxf(m, cm);
-    const float b = isinf(m) ? 0.f : m;
-    s *= __builtin_amdgcn_exp2f((base - b) * c);
-    base = b;
 #pragma unroll
-    for (int j = 0; j < kVE<T>; ++j) s += __builtin_amdgcn_exp2f((f[j] - b) * c);
-  });
-  // (a row of -inf: log 0; one with +inf: log inf; NaN stays)
-  float all = block_fold<BLOCK>(m, reinterpret_cast<float*>(red), MaxOp());
-  if (isinf(all)) all = 0.f;
-  s *= __builtin_amdgcn_exp2f((base - all) * c);
-  const double sum = block_fold<BLOCK>((double)s, red, SumOp());
-  if (threadIdx.x == 0) {
-    lse[r] = (float)((double)all * inv_t + log(sum));
-    found = 0;
-    bound = 0;
+    for (int j = 0; j < VE; ++j) s += term(f[j], c, base);
+    return cm;
+  };
+  // the logits of a chunk that reach a bound (no NaN among them); false once the list is full.
+  // (compared as they are: most of a wave's chunks hold one such logit or none)
+  auto collect = [&](int ch, const float* f, float low) {
+    bool room = true;
+#pragma unroll
+    for (int j = 0; j < VE; ++j)
+      if (f[j] >= low) {
+        const uint32_t at = atomicAdd(&found, 1u);
+        if (at < kList) list[at] = order_key(f[j], ch * VE + j);
+        else room = false;
+      }
+    return room;
+  };
+  if constexpr (NC > 0) {
+    row.each([&](int, const float* f, auto) {
+      first_base<VE>(base, f, c);
+      take(f);
+    });
+    if (threadIdx.x == 0) found = who_n = 0;
+  } else {
+    constexpr int A = 4, U = 2;   // chunks of the first part; loads in flight after it
+    uint4 v[A], next[U];
+    float f[VE];
+    const int t = threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < A; ++j) v[j] = load_chunk(row.p, min(t + j * BLOCK, row.n - 1), V);
+    auto fetch = [&](int at) {
+#pragma unroll
+      for (int j = 0; j < U; ++j) next[j] = load_chunk(row.p, min(at + j * BLOCK, row.n - 1), V);
+    };
+    fetch(t + A * BLOCK);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < A; ++j)
+      if (t + j * BLOCK < row.n) {
+        unpack(v[j], f, T());
+        first_base<VE>(base, f, c);
+        take(f);
+      }
+    maxima[t] = order_bits(m);
+    if (t == 0) found = who_n = 0;
+    __syncthreads();
+    if (t < 64) {
+      const float share = k * fminf(1.f, A * BLOCK / (float)row.n);
+      const int j = row.n > A * BLOCK ? (int)(share + 3.f * sqrtf(share)) + 3 : k;
+      const uint32_t least = bound_of_maxima<BLOCK>(maxima, min(j, BLOCK - 1), j / 8 + 2);
+      if (t == 0) bound = least;
+    }
+    __syncthreads();
+    const float low = float_of(bound);
+    // (nothing is put down for a bound of -inf: a masked part)
+    bool room = low > -INFINITY;
+#pragma unroll
+    for (int j = 0; j < A; ++j)
+      if (t + j * BLOCK < row.n) {
+        unpack(v[j], f, T());
+        if (room && chunk_max<VE>(f, -INFINITY) >= low) room = collect(t + j * BLOCK, f, low);
+      }
+    for (int ch = t + A * BLOCK; ch < row.n; ch += U * BLOCK) {
+#pragma unroll
+      for (int j = 0; j < U; ++j) v[j] = next[j];
+      fetch(ch + U * BLOCK);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < U; ++j)
+        if (ch + j * BLOCK < row.n) {
+          unpack(v[j], f, T());
+          if (take(f) >= low && room) room = collect(ch + j * BLOCK, f, low);
+        }
+    }
+    __syncthreads();   // (the first part's bound was read; maxima are written again)
   }
   const uint32_t mine = order_bits(m);
   maxima[threadIdx.x] = mine;
+  const float wb = wave_fold(base, MaxOp());
+  const float ws = wave_fold(s * __builtin_amdgcn_exp2f(base - wb), SumOp());
+  m = wave_fold(m, MaxOp());
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = {m, wb, ws};
   __syncthreads();
-
-  bool few = k <= BLOCK / 4 * 3 && sum == sum;   // (a thread's maximum passes over NaN)
-  if (few) {
-    if (threadIdx.x < 64) {
-      const uint32_t b = bound_of_maxima<BLOCK>(maxima, k);
-      if (threadIdx.x == 0) bound = b;
-    }
-    __syncthreads();
-    const uint32_t b = bound;
-    if (mine >= b) {
-      row.each([&](int ch, const float* f) {
+  // (a wave's part a lane: every wave joins them for itself)
+  const auto mp = part[threadIdx.x & (NW - 1)];
+  float all = wave_fold<NW>(mp.m, MaxOp());
+  const float b = wave_fold<NW>(mp.base, MaxOp());
+  double sum = wave_fold<NW>((double)mp.s * __builtin_amdgcn_exp2f(mp.base - b), SumOp());
+  bool finite = true;   // no NaN in the row
+  if (sum > 0 && sum < kMost) {
+    if (threadIdx.x == 0) lse[r] = (float)(((double)b + log2(sum)) * 0.6931471805599453);
+  } else {
+    // (a row of -inf: log 0; one with +inf: log inf; NaN stays)
+    if (isinf(all)) all = 0.f;
+    s = 0.f;
+    row.each([&](int, const float* f, auto) {
 #pragma unroll
-        for (int j = 0; j < kVE<T>; ++j) {
-          const int idx = ch * kVE<T> + j;
-          if (idx < V && order_bits(f[j]) >= b) {
-            const uint32_t at = atomicAdd(&found, 1u);
-            if (at < kList) list[at] = order_key(f[j], idx);
-          }
-        }
-      });
+      for (int j = 0; j < kVE<T>; ++j) s += term_at(f[j], all, c);
+    });
+    sum = block_fold<BLOCK>((double)s, red, SumOp());
+    finite = sum == sum;
+    if (threadIdx.x == 0) lse[r] = (float)((double)all * inv_t + log(sum));
+  }
+
+  bool few = finite && (int)found >= k && found <= kList;
+  if (!few && finite && k <= BLOCK / 4 * 3) {   // (a thread's maximum passes over NaN)
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      const uint32_t v = bound_of_maxima<BLOCK>(maxima, k, k / 4 + 8);
+      if (threadIdx.x == 0) bound = v, found = 0;
     }
     __syncthreads();
-    few = found <= kList;
+    const uint32_t least = bound;
+    const float low = float_of(least);
+    // (a bound of -inf would take in what pads the row's last chunk)
+    if (mine >= least && low > -INFINITY) who[atomicAdd(&who_n, 1u)] = threadIdx.x;
+    __syncthreads();
+    // the chunks of those threads, read again by all threads at once
+    const int per = (row.n + BLOCK - 1) / BLOCK, items = (int)who_n * per;
+    for (int w = threadIdx.x; w < items; w += BLOCK) {
+      const int ch = who[w / per] + w % per * BLOCK;
+      if (ch >= row.n) continue;
+      float f[VE];
+      unpack(load_chunk(row.p, ch, V), f, T());
+      collect(ch, f, low);
+    }
+    __syncthreads();
+    few = (int)found >= k && found <= kList;
   }
   if (!few) {
     __syncthreads();
     if (threadIdx.x == 0) found = 0;
     const uint64_t b = bound_of_keys(row, k, reinterpret_cast<int*>(red));
     __syncthreads();
-    row.each([&](int ch, const float* f) {
+    row.each([&](int ch, const float* f, auto) {
 #pragma unroll
       for (int j = 0; j < kVE<T>; ++j) {
         const int idx = ch * kVE<T> + j;
@@ -303,13 +472,19 @@ __global__ __launch_bounds__(BLOCK) void top_logits_kernel(const T* __restrict__
     });
     __syncthreads();
   }
-  // a candidate's place is the number of candidates before it
+  // a candidate's place is the number of candidates before it, counted by `parts` lanes each
   const int n = (int)found;
-  for (int i = threadIdx.x; i < n; i += BLOCK) {
-    const uint64_t key = list[i];
+  int parts = 1;
+  while (parts < 64 && 2 * parts * n <= BLOCK) parts *= 2;
+  const int part_of = threadIdx.x & (parts - 1);
+  for (int i0 = 0; i0 < n; i0 += BLOCK / parts) {
+    const int i = i0 + threadIdx.x / parts;
+    const uint64_t key = i < n ? list[i] : 0;
     int at = 0;
-    for (int j = 0; j < n; ++j) at += list[j] > key;
-    if (at < k) {
+#pragma unroll 8
+    for (int j = part_of; j < n; j += parts) at += list[j] > key;
+    for (int o = 1; o < parts; o *= 2) at += __shfl_xor(at, o, 64);
+    if (i < n && at < k && part_of == 0) {
       const int idx = key_index(key);
       values[r * k + at] = row.p[idx];
       indices[r * k + at] = idx;
@@ -347,7 +522,7 @@ __global__ __launch_bounds__(256) void top_small_kernel(const T* __restrict__ z,
 }
 
 // ------------------------------------------------------------------------------ distill_loss
-// Row of the loss, with q = softmax(z/T), e_j = exp((z_j - max z)/T), s = sum e:
+// Row of the loss, with q = softmax(z/T), e_j = exp(z_j/T) and s = sum e, both relative to a base:
 //   KD   = sum_k p_k (log p_k - log q_k) + rest (log rest - log q_rest)
 //   loss = alpha T^2 KD + (1 - alpha) (lse(z) - z_y)
 //   d/dz_j = e_j A - [not kept] e_j B - [kept] alpha T p_j + (1 - alpha)(softmax(z)_j - [j = y])
@@ -358,194 +533,284 @@ __global__ __launch_bounds__(256) void top_small_kernel(const T* __restrict__ z,
 //
 // A bit a class marks the kept ones (LDS, V / 8 bytes). It gives s_rest, and finds an index that
 // a row names twice: its entries are then gathered for each of them.
+//
+// The label's softmax is at temperature 1. Where T is 2 or 4 its exponentials are powers of those at
+// T, which saves the second quarter-rate instruction of a class and pass.
+struct Sums {
+  float base, base1;         // at T, at temperature 1
+  float rest, kept, one;     // of e over the classes not kept, the kept ones; of all at 1
+};
+
 template <typename T, int BLOCK, int NC, bool GRAD>
-__global__ __launch_bounds__(BLOCK) void distill_kernel(DistillArgs a, float c_t, float c_1) {
+__global__ __launch_bounds__(BLOCK)
+__attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void distill_kernel(DistillArgs a, float c_t) {
   extern __shared__ char smem[];
+  constexpr int NW = BLOCK / 64, VE = kVE<T>;
+  constexpr float kLog2e = 1.4426950408889634f;
+  constexpr double kLn2 = 0.6931471805599453;
   __shared__ double red[16];
-  __shared__ int flags[4];   // kept entries, an index twice, an index past the classes
+  __shared__ Sums part[NW];
+  __shared__ double side[3];   // the teacher's side: sum p, rest, sum p log p
+  __shared__ int flags[4];     // kept entries with mass, an index twice, an index past the classes
   const int64_t r = blockIdx.x;
-  const int V = a.V, K = a.K, t = threadIdx.x;
+  const int V = a.V, K = a.K, t = threadIdx.x, wave = t >> 6;
   double* p = reinterpret_cast<double*>(smem);          // [K] the teacher's probabilities
-  int* cls = reinterpret_cast<int*>(p + K);             // [K] their classes, -1: not kept
+  float* zk = reinterpret_cast<float*>(p + K);          // [K] the student's logits there
+  int* cls = reinterpret_cast<int*>(zk + K);            // [K] their classes, -1: not kept
   uint32_t* mark = reinterpret_cast<uint32_t*>(cls + K);
   const uint8_t* mark8 = reinterpret_cast<const uint8_t*>(mark);
-  const int words = (V + 31) / 32;
+  const T* zr = reinterpret_cast<const T*>(a.z) + r * a.ld;
 
-  for (int i = t; i < words; i += BLOCK) mark[i] = 0;
+  Row<T, BLOCK, NC> row;
+  row.load(zr, V);
+  int64_t y = a.target ? a.target[r] : a.ignore_index;
+  const bool label = a.target && y != a.ignore_index && a.alpha != 1.0;
+  bool poison = label && (y < 0 || y >= V);
+  if (poison || !label) y = 0;
+  const float zy = to_f(zr[y]);
+  const float lse = a.tail ? a.lse[r] : 0.f;
+
+  for (int i = t; i < (V + 31) / 32; i += BLOCK) mark[i] = 0;
   if (t < 4) flags[t] = 0;
   __syncthreads();
-
-  // ---- the teacher's side
-  double tmax = -INFINITY;
-  int kept = 0, twice = 0, bad = 0;
+  int mass_here = 0, twice = 0, bad = 0;
   for (int k = t; k < K; k += BLOCK) {
     const int64_t at = r * K + k;
     const int64_t idx = a.index64 ? reinterpret_cast<const int64_t*>(a.indices)[at]
                                   : (int64_t) reinterpret_cast<const int32_t*>(a.indices)[at];
-    double v = a.value_type == LOGIT_F32 ? (double)reinterpret_cast<const float*>(a.values)[at]
-               : a.value_type == LOGIT_BF16
-                   ? (double)to_f(reinterpret_cast<const bf16*>(a.values)[at])
-                   : (double)to_f(reinterpret_cast<const f16*>(a.values)[at]);
-    int j = -1;
+    const float v = a.value_type == LOGIT_F32 ? reinterpret_cast<const float*>(a.values)[at]
+                    : a.value_type == LOGIT_BF16
+                        ? to_f(reinterpret_cast<const bf16*>(a.values)[at])
+                        : to_f(reinterpret_cast<const f16*>(a.values)[at]);
+    const bool in = idx >= 0 && idx < V;
     if (idx >= V) bad = 1;
-    if (idx >= 0 && idx < V) {
-      j = (int)idx;
-      const uint32_t bit = 1u << (j & 31);
-      if (atomicOr(&mark[j >> 5], bit) & bit) twice = 1;
-      v /= a.temp;
-      kept = 1;
-      tmax = v != v ? v : fmax(tmax, v);
+    if (in) {
+      const uint32_t bit = 1u << (idx & 31);
+      if (atomicOr(&mark[idx >> 5], bit) & bit) twice = 1;
+      mass_here |= a.tail || v != -INFINITY;
+      zk[k] = to_f(zr[idx]);
     }
-    cls[k] = j;
-    p[k] = j < 0 ? -INFINITY : v;
+    cls[k] = in ? (int)idx : -1;
+    p[k] = in ? (double)v / a.temp : -INFINITY;
   }
-  if (kept) atomicOr(&flags[0], 1);
-  if (twice) atomicOr(&flags[1], 1);
-  if (bad) atomicOr(&flags[2], 1);
-  int64_t y = a.target ? a.target[r] : a.ignore_index;
-  const bool label = a.target && y != a.ignore_index && a.alpha != 1.0;
-  bool poison = label && (y < 0 || y >= V);
-  if (poison) y = 0;
-  tmax = block_fold<BLOCK>(tmax, red, MaxOp());
+  if (mass_here) flags[0] = 1;
+  if (twice) flags[1] = 1;
+  if (bad) flags[2] = 1;
   __syncthreads();
   poison |= flags[2] != 0;
   // a teacher's row without mass (nothing kept, or -inf alone) has no part in the loss
-  const double part = a.tail ? (double)a.lse[r] : tmax;
-  const bool kd = flags[0] != 0 && a.alpha != 0.0 && part != -INFINITY;
-
-  const T* zr = reinterpret_cast<const T*>(a.z) + r * a.ld;
+  const bool kd = flags[0] != 0 && a.alpha != 0.0 && lse != -INFINITY;
   T* dr = GRAD ? reinterpret_cast<T*>(a.dz) + r * V : nullptr;
-  constexpr int VE = kVE<T>;
-  const int nchunk = (V + VE - 1) / VE;
-  if (!kd && !label && !poison) {   // no term: the row's logits are not looked at
-    if (t == 0) a.row_loss[r] = 0.f;
-    if constexpr (GRAD) {
-      float f[VE] = {};
-      for (int c = t; c < nchunk; c += BLOCK) store_chunk(dr, c, V, f);
-    }
-    return;
-  }
-  if (poison) {
-    if (t == 0) a.row_loss[r] = __builtin_nanf("");
+  if (poison || (!kd && !label)) {   // without a term the row's logits do not count
+    const float v = poison ? __builtin_nanf("") : 0.f;
+    if (t == 0) a.row_loss[r] = v;
     if constexpr (GRAD) {
       float f[VE];
-      for (int j = 0; j < VE; ++j) f[j] = __builtin_nanf("");
-      for (int c = t; c < nchunk; c += BLOCK) store_chunk(dr, c, V, f);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) f[j] = v;
+      for (int c = t; c * VE < V; c += BLOCK) store_chunk(dr, c, V, f);
     }
     return;
   }
 
-  double mass = 0, rest = 0, kd_loss = 0;
-  if (kd) {
-    double lt = part;
+  // ---- the teacher's side, by the first wave (the others go on)
+  if (wave == 0 && kd) {
+    double lt = lse;
     if (!a.tail) {
-      double s = 0;
-      for (int k = t; k < K; k += BLOCK) s += cls[k] < 0 ? 0.0 : exp(p[k] - tmax);
-      lt = tmax + log(block_fold<BLOCK>(s, red, SumOp()));
+      double m = -INFINITY, s = 0;
+      for (int k = t; k < K; k += 64) m = p[k] != p[k] ? p[k] : fmax(m, p[k]);
+      m = wave_fold(m, MaxOp());
+      for (int k = t; k < K; k += 64) s += cls[k] < 0 ? 0.0 : exp(p[k] - m);
+      lt = m + log(wave_fold(s, SumOp()));
     }
-    double s = 0;
-    for (int k = t; k < K; k += BLOCK) {
-      if (cls[k] < 0) {
-        p[k] = 0;
-        continue;
-      }
-      const double lp = p[k] - lt, pk = exp(lp);
+    double s = 0, plogp = 0;
+    for (int k = t; k < K; k += 64) {
+      const double lp = p[k] - lt, pk = cls[k] < 0 ? 0.0 : exp(lp);
       p[k] = pk;
       s += pk;
-      if (pk > 0) kd_loss += pk * lp;
+      if (pk > 0) plogp += pk * lp;
     }
-    mass = block_fold<BLOCK>(s, red, SumOp());
+    s = wave_fold(s, SumOp());
+    plogp = wave_fold(plogp, SumOp());
+    double rest = 0;
     if (a.tail) {
-      int n = 0;
-      for (int i = t; i < words; i += BLOCK) n += __popc(mark[i]);
-      n = block_fold<BLOCK>(n, reinterpret_cast<int*>(red), SumOp());
-      rest = n < V ? 1.0 - mass : 0.0;
+      bool other = true;   // is any class not kept?
+      if (K >= V) {
+        int n = 0;
+        for (int i = t; i < (V + 31) / 32; i += 64) n += __popc(mark[i]);
+        other = wave_fold(n, SumOp()) < V;
+      }
+      rest = other ? 1.0 - s : 0.0;
       if (rest < kDistillRest) rest = 0.0;
     }
+    if (t == 0) side[0] = s, side[1] = rest, side[2] = plogp;
   }
 
-  // ---- the student's side
-  Row<T, BLOCK, NC> row;
-  row.load(zr, V);
-  float m = -INFINITY;
-  row.each([&](int, const float* f) {
+  // ---- the student's sums. power: exponentials at temperature 1 as that power of those at T
+  const bool one = label && (!kd || a.temp != 1.0);   // a softmax at temperature 1 of its own
+  const bool two = one && kd;
+  const float ct = kd ? c_t : kLog2e;
+  const int power = two ? (a.temp == 2.0 ? 2 : a.temp == 4.0 ? 4 : 0) : 0;
+  const bool tail = kd && a.tail;
+  Sums s = {kNoBase, kNoBase, 0.f, 0.f, 0.f};
+  float base1 = kNoBase;
+  // e: the chunk's exponentials at T
+  auto add = [&](int c, const float* e) {
+    float sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < VE; ++j) m = fmaxf(m, f[j]);
-  });
-  m = block_fold<BLOCK>(m, reinterpret_cast<float*>(red), MaxOp());
-  const bool one = label && (!kd || c_t != c_1);   // softmax at temperature 1 of its own
-  const bool tail = kd && rest > 0;
-  const float ct = kd ? c_t : c_1;
-  float s_t = 0.f, s_k = 0.f, s_1 = 0.f;
-  row.each([&](int c, const float* f) {
-    float e[VE], sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < VE; ++j) {
-      e[j] = __builtin_amdgcn_exp2f((f[j] - m) * ct);
-      sum += e[j];
-    }
+    for (int j = 0; j < VE; ++j) sum += e[j];
     const uint32_t bits = tail ? (mark8[c * VE >> 3] >> (c * VE & 7)) & ((1u << VE) - 1) : 0;
     if (bits) {
       float in = 0.f, out = 0.f;
 #pragma unroll
       for (int j = 0; j < VE; ++j) (bits >> j & 1 ? in : out) += e[j];
-      s_k += in;
+      s.kept += in;
       sum = out;
     }
-    s_t += sum;
-    if (one && kd) {
+    s.rest += sum;
+    if (power == 2) {
 #pragma unroll
-      for (int j = 0; j < VE; ++j) s_1 += __builtin_amdgcn_exp2f((f[j] - m) * c_1);
+      for (int j = 0; j < VE; ++j) s.one = fmaf(e[j], e[j], s.one);
+    } else if (power == 4) {
+#pragma unroll
+      for (int j = 0; j < VE; ++j) s.one = fmaf(e[j] * e[j], e[j] * e[j], s.one);
+    }
+  };
+  row.each([&](int c, const float* f, auto) {
+    first_base<VE>(s.base, f, ct);
+    float e[VE];
+#pragma unroll
+    for (int j = 0; j < VE; ++j) e[j] = term(f[j], ct, s.base);
+    add(c, e);
+    if (two && !power) {
+      first_base<VE>(base1, f, kLog2e);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) s.one += term(f[j], kLog2e, base1);
     }
   });
-  const double left = block_fold<BLOCK>((double)s_t, red, SumOp());
-  double total = left;
-  if (tail) total += block_fold<BLOCK>((double)s_k, red, SumOp());
-  double total1 = total;
-  if (one && kd) total1 = block_fold<BLOCK>((double)s_1, red, SumOp());
-  if (kd) {
-    // (differences to the maximum: a row of the type's lowest value has no digits left beside it)
-    for (int k = t; k < K; k += BLOCK)
-      if (p[k] > 0) kd_loss -= p[k] * (((double)to_f(zr[cls[k]]) - (double)m) / a.temp);
-    kd_loss = block_fold<BLOCK>(kd_loss, red, SumOp());
+  if (power) base1 = s.base * power;
+  // sums of the threads, in a fixed order: each wave's at its own base, then all of them
+  const float wb = wave_fold(s.base, MaxOp()), wb1 = wave_fold(base1, MaxOp());
+  auto join = [&](float scale, float scale1) {
+    const Sums w = {wb, wb1, wave_fold(s.rest * scale, SumOp()), wave_fold(s.kept * scale, SumOp()),
+                    wave_fold(s.one * scale1, SumOp())};
+    __syncthreads();
+    if ((t & 63) == 0) part[wave] = w;
+    __syncthreads();
+  };
+  join(__builtin_amdgcn_exp2f(s.base - wb), two ? __builtin_amdgcn_exp2f(base1 - wb1) : 0.f);
+  // (a wave's part a lane: every wave joins them for itself)
+  Sums v = part[t & (NW - 1)];
+  const float b = wave_fold<NW>(v.base, MaxOp()), b1 = wave_fold<NW>(v.base1, MaxOp());
+  double left = 0, inner = 0, total1 = 0;
+  auto total = [&](float scale, float scale1) {
+    left = wave_fold<NW>((double)v.rest * scale, SumOp());
+    if (tail) inner = wave_fold<NW>((double)v.kept * scale, SumOp());
+    if (two) total1 = wave_fold<NW>((double)v.one * scale1, SumOp());
+  };
+  total(__builtin_amdgcn_exp2f(v.base - b), __builtin_amdgcn_exp2f(v.base1 - b1));
+  // plain: exponentials against the row's maximum, for both temperatures
+  const double sum = left + inner;
+  const bool plain = !(sum > 0 && sum < kMost && (!two || (total1 > 0 && total1 < kMost)));
+  float m = 0.f;
+  if (plain) {
+    m = -INFINITY;
+    row.each([&](int, const float* f, auto) { m = chunk_max<VE>(f, m); });
+    m = block_fold<BLOCK>(m, reinterpret_cast<float*>(red), MaxOp());
+    s = {};
+    row.each([&](int c, const float* f, auto) {
+      float e[VE];
+#pragma unroll
+      for (int j = 0; j < VE; ++j) e[j] = term_at(f[j], m, ct);
+      add(c, e);
+      if (two && !power) {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) s.one += term_at(f[j], m, kLog2e);
+      }
+    });
+    join(1.f, 1.f);
+    v = part[t & (NW - 1)];
+    total(1.f, 1.f);
   }
+  const double all = left + inner;
+  if (!two) total1 = all;
+  const double mass = kd ? side[0] : 0, rest = kd ? side[1] : 0;
   const double at2 = a.alpha * a.temp;
-  if (t == 0) {
-    double loss = 0;
+
+  if (wave == 0) {
+    // log2 of a class's share, from the same constants as its exponential
+    double kl = 0;
     if (kd) {
-      // kd_loss holds sum p (log p - (z - max)/T); log q = (z - max)/T - log s
-      loss = kd_loss + mass * log(total);
-      if (tail) loss += rest * (log(rest) - log(left / total));
-      loss *= at2 * a.temp;
+      for (int k = t; k < K; k += 64) {
+        if (!(p[k] > 0)) continue;
+        const double x = plain ? ((double)zk[k] - (double)m) * (double)ct
+                               : (double)zk[k] * (double)ct - (double)b;
+        kl -= p[k] * x;
+      }
+      kl = wave_fold(kl, SumOp()) * kLn2 + side[2] + mass * log(all);
+      if (rest > 0) kl += rest * (log(rest) - log(left / all));
     }
-    if (label) loss += (1 - a.alpha) * ((double)m - (double)to_f(zr[y]) + log(total1));
-    a.row_loss[r] = (float)loss;
+    if (t == 0) {
+      double loss = kd ? kl * at2 * a.temp : 0;
+      if (label) {
+        const float c1 = two ? kLog2e : ct;
+        const double x = plain ? ((double)zy - (double)m) * (double)c1
+                               : (double)zy * (double)c1 - (double)(two ? b1 : b);
+        loss += (1 - a.alpha) * (log(total1) - x * kLn2);
+      }
+      a.row_loss[r] = (float)loss;
+    }
   }
   if constexpr (!GRAD) return;
 
   const double gs = a.grad_scale;
-  const double A = kd ? gs * at2 * (mass + rest) / total : 0.0;
-  const double B = tail && left > 0 ? gs * at2 * rest / left : 0.0;
+  const double A = kd ? gs * at2 * (mass + rest) / all : 0.0;
+  const double B = rest > 0 && left > 0 ? gs * at2 * rest / left : 0.0;
   const double D = label ? gs * (1 - a.alpha) / total1 : 0.0;
-  const bool both = kd && one;
-  const float ca = (float)(both ? A - B : A - B + D), cd = (float)D;
-  row.each([&](int c, const float* f) {
-    float d[VE];
+  const float ca = (float)(two ? A - B : A - B + D), cd = (float)D;
+  if (plain) {
+    row.each([&](int c, const float* f, auto whole) {
+      float g[VE];
 #pragma unroll
-    for (int j = 0; j < VE; ++j) {
-      d[j] = ca * __builtin_amdgcn_exp2f((f[j] - m) * ct);
-      if (both) d[j] += cd * __builtin_amdgcn_exp2f((f[j] - m) * c_1);
-    }
-    store_chunk(dr, c, V, d);
-  });
+      for (int j = 0; j < VE; ++j) {
+        g[j] = ca * term_at(f[j], m, ct);
+        if (two) g[j] += cd * term_at(f[j], m, kLog2e);
+      }
+      store_chunk<NC == 0>(dr, c, V, g, whole);
+    });
+  } else {
+    row.each([&](int c, const float* f, auto whole) {
+      float g[VE];
+#pragma unroll
+      for (int j = 0; j < VE; ++j) g[j] = term(f[j], ct, b);
+      if (!two) {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) g[j] *= ca;
+      } else if (power == 2) {
+        // (A - B) e + D e^2
+#pragma unroll
+        for (int j = 0; j < VE; ++j) g[j] *= fmaf(cd, g[j], ca);
+      } else if (power == 4) {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) g[j] *= fmaf(cd * g[j], g[j] * g[j], ca);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) g[j] = fmaf(cd, term(f[j], kLog2e, b1), ca * g[j]);
+      }
+      store_chunk<NC == 0>(dr, c, V, g, whole);
+    });
+  }
   // the kept classes and the label's, after the plain values above are written
   __syncthreads();
   const bool dup = flags[1] != 0;
-  auto fix = [&](int j, double pk) {
-    const double z = (double)to_f(zr[j]) - (double)m;
+  auto fix = [&](int j, float z, double share, double pk) {
     double g = -gs * at2 * pk;
-    if (kd) g += A * exp(z / a.temp);
-    if (label) g += D * exp(z) - (j == (int)y ? gs * (1 - a.alpha) : 0.0);
+    if (kd) g += share * (plain ? term_at(z, m, ct) : term(z, ct, b));
+    if (label) {
+      const float c1 = two ? kLog2e : ct;
+      g += D * (plain ? term_at(z, m, c1) : term(z, c1, two ? b1 : b));
+      if (j == (int)y) g -= gs * (1 - a.alpha);
+    }
     dr[j] = static_cast<T>((float)g);
   };
   if (kd) {
@@ -557,15 +822,10 @@ __global__ __launch_bounds__(BLOCK) void distill_kernel(DistillArgs a, float c_t
         for (int i = 0; i < K; ++i)
           if (cls[i] == cls[k]) pk += p[i];
       }
-      fix(cls[k], pk);
+      fix(cls[k], zk[k], A, pk);
     }
   }
-  if (label && t == 0 && !(kd && (mark[y >> 5] >> (y & 31) & 1))) {
-    const double z = (double)to_f(zr[y]) - (double)m;
-    double g = D * exp(z) - gs * (1 - a.alpha);
-    if (kd) g += (A - B) * exp(z / a.temp);
-    dr[y] = static_cast<T>((float)g);
-  }
+  if (label && t == 0 && !(kd && (mark[y >> 5] >> (y & 31) & 1))) fix((int)y, zy, A - B, 0.0);
 }
 
 __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restrict__ v, int64_t n,
@@ -595,19 +855,24 @@ __global__ __launch_bounds__(256) void scale_rows_kernel(T* __restrict__ dz, int
   }
 }
 
-// Threads and register chunks of a row: calls fn<BLOCK, NC>. again: long rows are read again
-template <typename T, typename F>
-void pick_row(int V, bool again, F&& fn) {
+// Threads and register chunks of a row of n chunks: calls fn<BLOCK, NC>. Up to 1024 chunks are held in
+// registers; longer rows are streamed by `threads` threads.
+template <typename F>
+void pick_row(int n, int threads, F&& fn) {
   using std::integral_constant;
-  const int n = (V + kVE<T> - 1) / kVE<T>;
-  if (n <= 64) fn(integral_constant<int, 64>(), integral_constant<int, 1>());
-  else if (n <= 256) fn(integral_constant<int, 64>(), integral_constant<int, 4>());
-  else if (n <= 1024) fn(integral_constant<int, 256>(), integral_constant<int, 4>());
-  else if (n <= 2048) fn(integral_constant<int, 256>(), integral_constant<int, 8>());
-  else if (again) fn(integral_constant<int, 1024>(), integral_constant<int, 0>());
-  else if (n <= 8192) fn(integral_constant<int, 1024>(), integral_constant<int, 8>());
-  else if (n <= 16384) fn(integral_constant<int, 1024>(), integral_constant<int, 16>());
-  else fn(integral_constant<int, 1024>(), integral_constant<int, 0>());
+  if (threads >= 1024) fn(integral_constant<int, 1024>(), integral_constant<int, 0>());
+  else if (n > 1024 && threads == 512) fn(integral_constant<int, 512>(), integral_constant<int, 0>());
+  else if (n > 1024) fn(integral_constant<int, 256>(), integral_constant<int, 0>());
+  else if (threads > 64 || n > 256) fn(integral_constant<int, 256>(), integral_constant<int, 4>());
+  else if (n > 64) fn(integral_constant<int, 64>(), integral_constant<int, 4>());
+  else fn(integral_constant<int, 64>(), integral_constant<int, 1>());
+}
+
+// Rows that do not fill the card (256 CUs of 2048 threads) take more threads each: top_logits of 509
+// rows of 32003 fp32, k 256, by 512 / 1024 threads 45 / 33 us.
+int few_rows(int64_t R, int threads) {
+  while (threads < 1024 && R * threads * 2 <= 256 * 2048) threads *= 2;
+  return threads;
 }
 
 template <typename F>
@@ -630,7 +895,16 @@ void top_logits_launch(const void* z, int type, int64_t ld, int64_t R, int V, in
                          reinterpret_cast<T*>(values), indices, lse);
       return;
     }
-    pick_row<T>(V, true, [&](auto block, auto nc) {
+    // k maxima of the threads bound the k largest while k is at most three quarters of them. Long rows:
+    // few threads a row leave more rows to hide a row's steps behind, until the first part (four
+    // chunks a thread) is too small a sample. 511 MB, k 64, by 256 / 512 / 1024 threads: 8388 x
+    // 32000 bf16 132 / 149 / 210 us, 2048 x 131072 bf16 132 / 108 / 118, fp32 (1023 MB) 247 / 198 / 185.
+    // Short rows, 67 MB by 64 / 256 threads: 33554 x 2000 bf16, k 100, 584 / 234 us; 67108 x 1000 bf16,
+    // k 100 (125 chunks: too few maxima), 744 / 1827.
+    const int n = (V + kVE<T> - 1) / kVE<T>;
+    const int threads = n <= 1024 ? (k > 48 && k <= 192 && 3 * n >= 4 * k ? 256 : 64)
+                        : few_rows(R, n <= 4096 && k <= 64 ? 256 : n <= 16384 && k <= 384 ? 512 : 1024);
+    pick_row(n, threads, [&](auto block, auto nc) {
       constexpr int BLOCK = decltype(block)::value, NC = decltype(nc)::value;
       hipLaunchKernelGGL((top_logits_kernel<T, BLOCK, NC>), dim3((uint32_t)R), dim3(BLOCK), 0, st,
                          reinterpret_cast<const T*>(z), ld, V, k, c, 1.0 / temp,
@@ -640,18 +914,26 @@ void top_logits_launch(const void* z, int type, int64_t ld, int64_t R, int V, in
 }
 
 void distill_launch(const DistillArgs& a, hipStream_t st) {
-  const float c_t = (float)(1.4426950408889634 / a.temp), c_1 = 1.4426950408889634f;
-  const size_t lds = (size_t)a.K * 12 + (size_t)((a.V + 31) / 32) * 4;
+  const float c_t = (float)(1.4426950408889634 / a.temp);
+  const size_t lds = (size_t)a.K * 16 + (size_t)((a.V + 31) / 32) * 4;
   pick_type(a.type, [&](auto tv) {
     using T = decltype(tv);
-    pick_row<T>(a.V, false, [&](auto block, auto nc) {
+    // The rows at work at once are read again for the gradient: with few threads a row there are more of
+    // them than the cache behind the L2s keeps (2048 x 131072 bf16 by 256 / 512 / 1024 threads 335 /
+    // 309 / 279 us; 16384 x 16384 275 / 263 / 402). The loss alone reads them once (8388 x 32000 bf16
+    // 110 / 124 / 192 us).
+    const int n = (a.V + kVE<T> - 1) / kVE<T>;
+    const int threads = n <= 1024 ? 64
+                                  : few_rows(a.R, a.dz ? (n <= 8192 ? 512 : 1024)
+                                                       : n <= 8192 ? 256 : 512);
+    pick_row(n, threads, [&](auto block, auto nc) {
       constexpr int BLOCK = decltype(block)::value, NC = decltype(nc)::value;
       if (a.dz)
         hipLaunchKernelGGL((distill_kernel<T, BLOCK, NC, true>), dim3((uint32_t)a.R), dim3(BLOCK),
-                           lds, st, a, c_t, c_1);
+                           lds, st, a, c_t);
       else
         hipLaunchKernelGGL((distill_kernel<T, BLOCK, NC, false>), dim3((uint32_t)a.R), dim3(BLOCK),
-                           lds, st, a, c_t, c_1);
+                           lds, st, a, c_t);
     });
   });
 }

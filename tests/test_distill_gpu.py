@@ -61,7 +61,10 @@ def test_top_logits(r, v, k, dtype):
 @pytest.mark.parametrize("v", [6, 300, 5000, 40000, 200000])
 def test_top_logits_hard_rows(v, dtype):
     k = min(v, 200)
-    z = make(12, v, dtype, 1)
+    z = make(15, v, dtype, 1)
+    z[12, :2 * v // 3] = -math.inf
+    z[13, :v // 3] = torch.finfo(dtype).min
+    z[14] = -torch.arange(v).to(dtype)
     z[0] = -math.inf
     z[1] = 1.0                                    # all equal
     z[2] = torch.randint(0, 3, (v,)).to(dtype)    # few values
@@ -78,7 +81,7 @@ def test_top_logits_hard_rows(v, dtype):
     top = PF.top_logits(z.cuda(), k)
     want = PF.top_logits(z, k)
     assert torch.equal(top.indices.cpu(), want.indices)
-    check_top(z[[0, 1, 2, 3, 5, 8, 11]], k)
+    check_top(z[[0, 1, 2, 3, 5, 8, 11, 12]], k)
     lse = top.lse.cpu()
     assert lse[0] == -math.inf and lse[5] == math.inf
     assert lse[4].isnan() and lse[10].isnan()
@@ -146,7 +149,9 @@ def test_distill(r, v, k, dtype, tail, labels, t):
     assert ((rows.cpu().double() - want).abs() <= tl + 2 * U * want.abs()).all()
     loss = PF.distill_loss(x, *args, reduction="sum", **kw)
     loss.backward(PF.unit_grad(loss))
-    assert abs(loss.item() - rows.double().sum().item()) <= U * rows.double().abs().sum().item() + 1e-30
+    # (the pass with a gradient may sum a row in another order than the one without: each row of it is
+    # held to the oracle's by the same bound, and their sum by the bounds' sum and its own rounding)
+    assert abs(loss.item() - want.sum().item()) <= r * tl + 3 * U * want.abs().sum().item()
     assert x.grad.dtype == dtype
     assert ((x.grad.cpu().double() - grad).abs() <= tg(dtype)).all()
     if r > 2 and labels:
