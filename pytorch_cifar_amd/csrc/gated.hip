@@ -187,28 +187,30 @@ __global__ __launch_bounds__(WM* WN * 64) void gated_kernel(GatedArgs a, int mt,
   if constexpr (kTermsQ) qb += ((int64_t)half * a.qseg + m0) * ES;
   else qb += (int64_t)m0 * a.ldq * ES;
 
-  auto issue = [&](int t, int buf) {
+  // K tile t: its first term and where it lies
+  struct Src {
+    int k0;
+    const char *q, *p, *u;
+  };
+  auto source = [&](int t) {
     const int seg = FORM == GATED_DX && t >= per_seg;
-    const int k0 = (t - (seg ? per_seg : 0)) * BK;
-    const char* q = qb + (kTermsQ ? (int64_t)k0 * a.ldq : (int64_t)k0 + seg * a.qseg) * ES;
-    const auto rq = make_rsrc(q, 0x7fffffffu);
-#pragma unroll
-    for (int i = 0; i < QP; ++i)
-      dma16(rq, &lds[buf][(i * NW + wave) * 1024], k0 + qk[i] < a.K ? qoff[i] : kOOB);
-    if constexpr (kFwd) {
-      const char* g = reinterpret_cast<const char*>(a.p0) + ((int64_t)n0 * a.ldp + k0) * ES;
-      const char* u = reinterpret_cast<const char*>(a.p1) + ((int64_t)n0 * a.ldp + k0) * ES;
-#pragma unroll
-      for (int i = 0; i < PP; ++i)
-        dma16(make_rsrc(up[i] ? u : g, 0x7fffffffu), &lds[buf][QB + (i * NW + wave) * 1024],
-              k0 + pk[i] < a.K ? poff[i] : kOOB);
+    Src s;
+    s.k0 = (t - (seg ? per_seg : 0)) * BK;
+    s.q = qb + (kTermsQ ? (int64_t)s.k0 * a.ldq : (int64_t)s.k0 + seg * a.qseg) * ES;
+    const int64_t at = (kFwd ? (int64_t)n0 * a.ldp + s.k0 : (int64_t)s.k0 * a.ldp + n0) * ES;
+    s.p = reinterpret_cast<const char*>(seg ? a.p1 : a.p0) + at;
+    s.u = reinterpret_cast<const char*>(a.p1) + at;   // (forward: the other weight)
+    return s;
+  };
+  constexpr int kPieces = QP + PP;
+  auto issue = [&](const Src& s, int buf, int i) {   // the wave's piece i of a tile
+    if (i < QP) {
+      dma16(make_rsrc(s.q, 0x7fffffffu), &lds[buf][(i * NW + wave) * 1024],
+            s.k0 + qk[i] < a.K ? qoff[i] : kOOB);
     } else {
-      const char* p = reinterpret_cast<const char*>(seg ? a.p1 : a.p0) +
-                      ((int64_t)k0 * a.ldp + n0) * ES;
-      const auto rp = make_rsrc(p, 0x7fffffffu);
-#pragma unroll
-      for (int i = 0; i < PP; ++i)
-        dma16(rp, &lds[buf][QB + (i * NW + wave) * 1024], k0 + pk[i] < a.K ? poff[i] : kOOB);
+      const int j = i - QP;
+      dma16(make_rsrc(kFwd && up[j] ? s.u : s.p, 0x7fffffffu), &lds[buf][QB + (j * NW + wave) * 1024],
+            s.k0 + pk[j] < a.K ? poff[j] : kOOB);
     }
   };
 
@@ -218,37 +220,93 @@ __global__ __launch_bounds__(WM* WN * 64) void gated_kernel(GatedArgs a, int mt,
 #pragma unroll
     for (int j = 0; j < MF; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
 
-  if (t0 < t1) issue(t0, 0);
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    if (t + 1 < t1) {
-      issue(t + 1, buf ^ 1);
-      wait_vmcnt<QP + PP>();
+  // A K tile is two steps of 64 bytes of terms. While a step's products run, the next step's
+  // fragments are read in the place of those that are done; between the last step of a tile and the
+  // first of the next stands the tile's one barrier: all waves have read the old buffer, which the
+  // tile after next then fills, and all pieces of the next have landed.
+  typename Mat<E>::frag q[MF], p[NF];
+  auto read_q = [&](int buf, int s, int j) {
+    return kTermsQ ? frag_terms<E>(lds[buf], wm * TM + 16 * j, s, lane)
+                   : frag_rows<E>(lds[buf], wm * TM + 16 * j, s, lane);
+  };
+  auto read_p = [&](int buf, int s, int i) {
+    return kTermsP ? frag_terms<E>(lds[buf] + QB, wn * TN + 16 * i, s, lane)
+                   : frag_rows<E>(lds[buf] + QB, wn * TN + 16 * i, s, lane);
+  };
+  // The step's products on q, p, the reads of the next behind the first of them (by the step's end
+  // they have long arrived), and, with `src`, the pieces of a later tile between them: issued all at
+  // once they would hold the products up until the last wave's have been taken.
+  auto step = [&](auto fill, int buf, int s, const Src& src, int to) {
+    typename Mat<E>::frag nq[MF], np[NF];
+    constexpr int kG = MF >= 4 ? MF / 2 : 1, kFrags = (NF + MF + kG - 1) / kG;
+    constexpr int kEach = (kPieces + MF - 1) / MF;
+#pragma unroll
+    for (int j = 0; j < MF; ++j) {
+#pragma unroll
+      for (int i = 0; i < NF; ++i) Mat<E>::mma(p[i], q[j], acc[i][j]);
+#pragma unroll
+      for (int r = j * kFrags; r < (j + 1) * kFrags; ++r) {
+        if (r < NF) np[r] = read_p(buf, s, r);
+        else if (r < NF + MF) nq[r - NF] = read_q(buf, s, r - NF);
+      }
+      if constexpr (decltype(fill)::value) {
+#pragma unroll
+        for (int i = j * kEach; i < (j + 1) * kEach && i < kPieces; ++i) issue(src, to, i);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 0; i < NF; ++i) p[i] = np[i];
+#pragma unroll
+    for (int j = 0; j < MF; ++j) q[j] = nq[j];
+  };
+  constexpr std::integral_constant<bool, true> kFill;
+  constexpr std::integral_constant<bool, false> kNoFill;
+  if (t0 < t1) {
+    const Src first = source(t0);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) issue(first, 0, i);
+    if (t0 + 1 < t1) {
+      const Src second = source(t0 + 1);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) issue(second, 1, i);
+      wait_vmcnt<kPieces>();
     } else {
       wait_vmcnt<0>();
     }
     raw_barrier();
-    const char* lq = lds[buf];
-    const char* lp = lds[buf] + QB;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      typename Mat<E>::frag q[MF], p[NF];
+    for (int i = 0; i < NF; ++i) p[i] = read_p(0, 0, i);
 #pragma unroll
-      for (int j = 0; j < MF; ++j)
-        q[j] = kTermsQ ? frag_terms<E>(lq, wm * TM + 16 * j, s, lane)
-                       : frag_rows<E>(lq, wm * TM + 16 * j, s, lane);
-#pragma unroll
-      for (int i = 0; i < NF; ++i)
-        p[i] = kTermsP ? frag_terms<E>(lp, wn * TN + 16 * i, s, lane)
-                       : frag_rows<E>(lp, wn * TN + 16 * i, s, lane);
-#pragma unroll
-      for (int i = 0; i < NF; ++i)
-#pragma unroll
-        for (int j = 0; j < MF; ++j) Mat<E>::mma(p[i], q[j], acc[i][j]);
-    }
-    // every wave has its fragments before the buffer is written again
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    for (int j = 0; j < MF; ++j) q[j] = read_q(0, 0, j);
+    // lgkmcnt(0): with a scalar load pending at the loop's entry every wait in it would be for all
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+  }
+  int t = t0;
+  auto turn = [&]() {   // between two tiles
+    __builtin_amdgcn_s_waitcnt(0x70);   // vmcnt(0) lgkmcnt(0): as the compiler knows it
     raw_barrier();
+  };
+  for (; t + 2 < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    const Src src = source(t + 2);
+    step(kNoFill, buf, 1, src, 0);
+    turn();
+    step(kFill, buf ^ 1, 0, src, buf);
+  }
+  if (t + 1 < t1) {
+    const int buf = (t - t0) & 1;
+    step(kNoFill, buf, 1, Src(), 0);
+    turn();
+    step(kNoFill, buf ^ 1, 0, Src(), 0);
+    ++t;
+  }
+  if (t < t1) {
+    step(kNoFill, (t - t0) & 1, 1, Src(), 0);
+#pragma unroll
+    for (int j = 0; j < MF; ++j)
+#pragma unroll
+      for (int i = 0; i < NF; ++i) Mat<E>::mma(p[i], q[j], acc[i][j]);
   }
 
   // ---- epilogue: lane holds columns 4 (lane >> 4) .. + 3 of row (lane & 15) of each 16 x 16 tile
