@@ -93,15 +93,35 @@ __device__ __forceinline__ typename Mat<E>::frag frag_terms(const char* lds, int
   }
 }
 
-__device__ __forceinline__ float act_val(float g, int act) { return apply_act(g, act); }
+// The reciprocal instruction (1 step) in the place of the quotient, ten instructions: the epilogue
+// takes a sigmoid of every hidden unit while the matrix cores stand still.
+__device__ __forceinline__ float sigmoid(float x) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504f));
+}
+__device__ __forceinline__ float act_val(float g, int act) {
+  if (act == ACT_SWISH) return g * sigmoid(g);
+  if (act == ACT_SIGMOID) return sigmoid(g);
+  return act == ACT_RELU ? fmaxf(g, 0.f) : g;
+}
+// act(g) and its slope
+__device__ __forceinline__ void act_both(float g, int act, float& v, float& slope) {
+  if (act == ACT_SWISH || act == ACT_SIGMOID) {
+    const float s = sigmoid(g);
+    v = act == ACT_SWISH ? g * s : s;
+    slope = act == ACT_SWISH ? fmaf(v, 1.f - s, s) : s * (1.f - s);
+  } else {
+    v = act == ACT_RELU ? fmaxf(g, 0.f) : g;
+    slope = act == ACT_RELU && !(g > 0.f) ? 0.f : 1.f;
+  }
+}
 
 // 4 consecutive outputs of a row at column n (N columns in all), at any alignment
 template <typename O>
-__device__ __forceinline__ void store4(O* row, int n, int N, const f32x4& v) {
+__device__ __forceinline__ void store4(O* row, int n, int N, const f32x4& v, bool whole) {
   O h[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) h[i] = static_cast<O>(v[i]);
-  if (n + 4 <= N) {
+  if (whole || n + 4 <= N) {
     __builtin_memcpy(row + n, h, sizeof(h));
   } else {
 #pragma unroll
@@ -311,48 +331,149 @@ __global__ __launch_bounds__(WM* WN * 64) void gated_kernel(GatedArgs a, int mt,
 
   // ---- epilogue: lane holds columns 4 (lane >> 4) .. + 3 of row (lane & 15) of each 16 x 16 tile
   const int cl = 4 * (lane >> 4);
-  if constexpr (kFwd) {
+  const int act = a.act;
+  auto put = [&](auto whole) {   // whole: all of the tile's rows and columns are there
+    constexpr bool W = decltype(whole)::value;
 #pragma unroll
     for (int j = 0; j < MF; ++j) {
       const int m = m0 + wm * TM + 16 * j + (lane & 15);
-      if (m >= a.M) continue;
+      if (!W && m >= a.M) continue;
+      const int64_t at = (int64_t)m * a.N;
+      if constexpr (kFwd) {
+        O* out = reinterpret_cast<O*>(a.out0) + at;
+        float* part = a.part ? a.part + ((int64_t)split * a.M + m) * 2 * a.N : nullptr;
 #pragma unroll
-      for (int i = 0; i < NF / 2; ++i) {
-        const int n = n0 + wn * (TN / 2) + 16 * i + cl;
-        const f32x4 g = acc[i][j], u = acc[i + NF / 2][j];
-        if (a.part) {
-          float* row = a.part + ((int64_t)split * a.M + m) * 2 * a.N;
-          store4(row, n, a.N, g);
-          store4(row + a.N, n, a.N, u);
-          continue;
+        for (int i = 0; i < NF / 2; ++i) {
+          const int n = n0 + wn * (TN / 2) + 16 * i + cl;
+          const f32x4 g = acc[i][j], u = acc[i + NF / 2][j];
+          if (part) {
+            store4(part, n, a.N, g, W);
+            store4(part + a.N, n, a.N, u, W);
+            continue;
+          }
+          if (a.save_g) {
+            store4(a.save_g + at, n, a.N, g, W);
+            store4(a.save_u + at, n, a.N, u, W);
+          }
+          f32x4 h;
+          if (act == ACT_SWISH) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = g[e] * sigmoid(g[e]) * u[e];
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = act_val(g[e], act) * u[e];
+          }
+          store4(out, n, a.N, h, W);
         }
-        f32x4 h;
+      } else {
+        const int64_t rows = (FORM == GATED_DW ? 2 : 1) * (int64_t)a.M;
+        float* part = a.part ? a.part + (split * rows + half * (int64_t)a.M + m) * a.N : nullptr;
+        O* out = reinterpret_cast<O*>(half ? a.out1 : a.out0) + at;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) h[e] = act_val(g[e], a.act) * u[e];
-        store4(reinterpret_cast<O*>(a.out0) + (int64_t)m * a.N, n, a.N, h);
-        if (a.save_g) {
-          store4(a.save_g + (int64_t)m * a.N, n, a.N, g);
-          store4(a.save_u + (int64_t)m * a.N, n, a.N, u);
+        for (int i = 0; i < NF; ++i) {
+          const int n = n0 + wn * TN + 16 * i + cl;
+          if (part) store4(part, n, a.N, acc[i][j], W);
+          else store4(out, n, a.N, acc[i][j], W);
         }
       }
     }
-  } else {
+  };
+  if (m0 + BM <= a.M && n0 + NH <= a.N) put(std::integral_constant<bool, true>());
+  else put(std::integral_constant<bool, false>());
+}
+
+// ------------------------------------------------------------------------ few rows (forward)
+// Up to 64 rows: the weights are read once, straight into the fragments' registers, and that read is
+// all the time there is. A workgroup has 16 hidden units of both weights; its waves take every NW-th
+// 64 bytes of the width, and their sums are joined in LDS, in order. The rows come from the caches
+// (every workgroup reads all of them).
+template <typename E, int MT, int NW>
+__global__ __launch_bounds__(NW * 64) void gated_few_kernel(GatedArgs a) {
+  constexpr int ES = sizeof(E), UB = 1, U = MT == 1 ? 4 : 2;   // 16-unit blocks; steps in flight
+  __shared__ f32x4 sums[NW][2 * UB * MT][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * 16 * UB;
+  const int64_t at = (int64_t)n0 * a.ldp * ES;
+  const auto rg = make_rsrc(reinterpret_cast<const char*>(a.p0) + at, 0x7fffffffu);
+  const auto ru = make_rsrc(reinterpret_cast<const char*>(a.p1) + at, 0x7fffffffu);
+  const auto rx = make_rsrc(a.q, 0x7fffffffu);
+  const int r = lane & 15, c = (lane >> 4) * 16;
+  uint32_t wo[UB], xo[MT];
 #pragma unroll
-    for (int j = 0; j < MF; ++j) {
-      const int m = m0 + wm * TM + 16 * j + (lane & 15);
-      if (m >= a.M) continue;
+  for (int i = 0; i < UB; ++i)
+    wo[i] = n0 + 16 * i + r < a.N ? (uint32_t)((16 * i + r) * a.ldp) * ES + c : kOOB;
 #pragma unroll
-      for (int i = 0; i < NF; ++i) {
-        const int n = n0 + wn * TN + 16 * i + cl;
-        if (a.part) {
-          const int64_t rows = (FORM == GATED_DW ? 2 : 1) * (int64_t)a.M;
-          store4(a.part + (split * rows + half * (int64_t)a.M + m) * a.N, n, a.N, acc[i][j]);
-        } else {
-          O* out = reinterpret_cast<O*>(half ? a.out1 : a.out0);
-          store4(out + (int64_t)m * a.N, n, a.N, acc[i][j]);
-        }
-      }
+  for (int i = 0; i < MT; ++i)
+    xo[i] = 16 * i + r < a.M ? (uint32_t)((16 * i + r) * a.ldq) * ES + c : kOOB;
+  const int bytes = a.K * ES, steps = (bytes + 63) / 64;
+
+  typedef int i32x4 __attribute__((ext_vector_type(4)));
+  typedef typename Mat<E>::frag frag;
+  struct Step {
+    i32x4 g[UB], u[UB], x[MT];
+  };
+  auto load = [&](Step& s, int i) {   // past the width: zeros
+    const int k = i * 64;
+    const bool in = k + c < bytes;
+#pragma unroll
+    for (int j = 0; j < UB; ++j) {
+      s.g[j] = __builtin_amdgcn_raw_buffer_load_b128(rg, in ? wo[j] : kOOB, k, 0);
+      s.u[j] = __builtin_amdgcn_raw_buffer_load_b128(ru, in ? wo[j] : kOOB, k, 0);
     }
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+      s.x[j] = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? xo[j] : kOOB, k, 0);
+  };
+  f32x4 acc[2 * UB][MT];
+#pragma unroll
+  for (int i = 0; i < 2 * UB; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
+  Step now[U], next[U];
+#pragma unroll
+  for (int j = 0; j < U; ++j) load(now[j], wave + j * NW);
+  for (int i = wave; i < steps; i += U * NW) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) load(next[j], i + (U + j) * NW);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int b = 0; b < UB; ++b) {
+          const frag x = __builtin_bit_cast(frag, now[j].x[m]);
+          Mat<E>::mma(__builtin_bit_cast(frag, now[j].g[b]), x, acc[b][m]);
+          Mat<E>::mma(__builtin_bit_cast(frag, now[j].u[b]), x, acc[UB + b][m]);
+        }
+#pragma unroll
+    for (int j = 0; j < U; ++j) now[j] = next[j];
+  }
+#pragma unroll
+  for (int i = 0; i < 2 * UB; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) sums[wave][i * MT + j][lane] = acc[i][j];
+  __syncthreads();
+  for (int b = wave; b < UB * MT; b += NW) {
+    const int i = b / MT, j = b % MT;
+    f32x4 g = sums[0][i * MT + j][lane], u = sums[0][(UB + i) * MT + j][lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) {
+      g += sums[w][i * MT + j][lane];
+      u += sums[w][(UB + i) * MT + j][lane];
+    }
+    const int m = 16 * j + (lane & 15), n = n0 + 16 * i + 4 * (lane >> 4);
+    if (m >= a.M) continue;
+    const int64_t to = (int64_t)m * a.N;
+    if (a.save_g) {
+      store4(a.save_g + to, n, a.N, g, false);
+      store4(a.save_u + to, n, a.N, u, false);
+    }
+    f32x4 h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = act_val(g[e], a.act) * u[e];
+    store4(reinterpret_cast<E*>(a.out0) + to, n, a.N, h, false);
   }
 }
 
@@ -416,8 +537,10 @@ __global__ __launch_bounds__(256) void gated_dact_kernel(const float* __restrict
 #pragma unroll
     for (int i = 0; i < PC; ++i) {
       const float df = static_cast<float>(d[i]);
-      dg[i] = static_cast<E>(df * uv[i] * act_grad(gv[i], act));
-      du[i] = static_cast<E>(df * act_val(gv[i], act));
+      float v, slope;
+      act_both(gv[i], act, v, slope);
+      dg[i] = static_cast<E>(df * uv[i] * slope);
+      du[i] = static_cast<E>(df * v);
     }
     E* row = out + m * 2 * Fp + f0;
     __builtin_memcpy(row, dg, 16);
@@ -460,36 +583,63 @@ uint32_t grid_for(int64_t n) { return (uint32_t)std::max<int64_t>(1, std::min<in
 
 constexpr int kCUs = 256;
 
-// 256 x 256 tiles where they fill the card at least once, 128 x 128 ones below
+constexpr int kFewRows = 64;
+
+// Tiles and splits of the sum by a model of the time in us, from measured times: a K tile of 64
+// (fp32: 32) terms takes a 256 x 256 tile 1.25 (fp32 7.6), a 128 x 128 tile alone on its compute unit
+// 0.65 (2.1) and two that share one 1.11 (3.9); a tile's start and end take 12 and 8; the partial sums
+// of splits are written and read at 4.5 TB/s by one more launch.
 struct Plan {
   bool big;
   int mt, nt, splits;
 };
 Plan plan(int form, int type, int M, int N, int K) {
-  Plan p{};
   const int halves = form == GATED_DW ? 2 : 1, nh = form == GATED_FWD ? 2 : 1;
-  auto tiles = [&](int b) { return (int64_t)halves * cdiv(M, b) * cdiv(N * nh, b); };
-  p.big = tiles(256) >= kCUs;
-  const int b = p.big ? 256 : 128;
-  p.mt = halves * cdiv(M, b);
-  p.nt = cdiv(N * nh, b);
-  const int nk = (form == GATED_DX ? 2 : 1) * cdiv(K, 128 / (type == GATED_F32 ? 4 : 2));
-  const int64_t t = (int64_t)p.mt * p.nt;
-  // few tiles: the sum is split until the card is filled once, to no less than 4 K tiles each
-  p.splits = 1;
-  if (t * 2 <= kCUs) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kCUs / t, nk / 4));
-  return p;
+  const bool f32 = type == GATED_F32;
+  const int nk = (form == GATED_DX ? 2 : 1) * cdiv(K, kRow / (f32 ? 4 : 2));
+  Plan best{};
+  double least = 0;
+  for (int big = 0; big < 2; ++big) {
+    const int b = big ? 256 : 128;
+    const int mt = halves * cdiv(M, b), nt = cdiv(N * nh, b);
+    for (int s = 1; s <= 16 && (s == 1 || nk / s >= 4); ++s) {
+      const int64_t n = (int64_t)mt * nt * s;
+      const double each = big ? (f32 ? 7.6 : 1.25) : n <= kCUs ? (f32 ? 2.1 : 0.65) : f32 ? 3.9 : 1.11;
+      const double rounds = (double)cdiv64(n, big || n <= kCUs ? kCUs : 2 * kCUs);
+      double us = rounds * (cdiv(nk, s) * each + (big ? 12 : 8));
+      if (s > 1) us += 5 + (double)M * N * halves * nh * 4 * (2 * s) / 4.5e6;
+      if (least == 0 || us < least) {
+        least = us;
+        best = {big != 0, mt, nt, s};
+      }
+    }
+  }
+  return best;
 }
 
 }  // namespace
 
-int gated_splits(int form, int type, int M, int N, int K) { return plan(form, type, M, N, K).splits; }
+int gated_splits(int form, int type, int M, int N, int K) {
+  if (form == GATED_FWD && M <= kFewRows) return 1;
+  return plan(form, type, M, N, K).splits;
+}
 
 int64_t gated_part_floats(int form, int M, int N) {
   return (int64_t)M * N * (form == GATED_DX ? 1 : 2);
 }
 
 void gated_launch(int form, int type, bool out_f32, const GatedArgs& a, hipStream_t st) {
+  if (form == GATED_FWD && a.M <= kFewRows) {
+    pick_type(type, [&](auto ev) {
+      using E = decltype(ev);
+      const dim3 grid((uint32_t)cdiv(a.N, 16));
+      if (a.M <= 16) hipLaunchKernelGGL((gated_few_kernel<E, 1, 4>), grid, dim3(256), 0, st, a);
+      else if (a.M <= 32) hipLaunchKernelGGL((gated_few_kernel<E, 2, 4>), grid, dim3(256), 0, st, a);
+      else if (a.M <= 48) hipLaunchKernelGGL((gated_few_kernel<E, 3, 4>), grid, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((gated_few_kernel<E, 4, 4>), grid, dim3(256), 0, st, a);
+    });
+    return;
+  }
   const Plan p = plan(form, type, a.M, a.N, a.K);
   const dim3 grid((uint32_t)(p.mt * p.nt), (uint32_t)a.splits);
   const int64_t n = (int64_t)a.M * a.N;
