@@ -386,9 +386,10 @@ __global__ __launch_bounds__(WM* WN * 64) void gated_kernel(GatedArgs a, int mt,
 // Up to 64 rows: the weights are read once, straight into the fragments' registers, and that read is
 // all the time there is. A workgroup has 16 hidden units of both weights; its waves take every NW-th
 // 64 bytes of the width, and their sums are joined in LDS, in order. The rows come from the caches
-// (every workgroup reads all of them).
+// (every workgroup reads all of them). One row, 4096 -> 10752 bf16 (176 MB): 38 us, 4.6 TB/s.
 template <typename E, int MT, int NW>
-__global__ __launch_bounds__(NW * 64) void gated_few_kernel(GatedArgs a) {
+__global__ __launch_bounds__(NW * 64) 
+__attribute__((amdgpu_waves_per_eu(MT < 4 ? 4 : 2))) void gated_few_kernel(GatedArgs a) {
   constexpr int ES = sizeof(E), UB = 1, U = MT == 1 ? 4 : 2;   // 16-unit blocks; steps in flight
   __shared__ f32x4 sums[NW][2 * UB * MT][64];
   const int lane = threadIdx.x & 63;
@@ -583,7 +584,13 @@ uint32_t grid_for(int64_t n) { return (uint32_t)std::max<int64_t>(1, std::min<in
 
 constexpr int kCUs = 256;
 
-constexpr int kFewRows = 64;
+// Rows up to which gated_few_kernel is taken: it reads all rows once a 16 hidden units, which by some
+// 30 rows is as much as the weights. In us, by it and by tiles: 4096 -> 10752 bf16 8 / 16 / 32 rows 40 /
+// 44 / 54 and 38, 2048 -> 5504 17 / 32 / 48 rows 15 / 17 / 21 and 19, 1024 -> 4096 6 / 7 / 8 and 16.
+bool few_rows(int type, int M, int N, int K) {
+  const double weights = 2.0 * N * K * (type == GATED_F32 ? 4 : 2);
+  return M <= 64 && weights * M <= 1.6e9;
+}
 
 // Tiles and splits of the sum by a model of the time in us, from measured times: a K tile of 64
 // (fp32: 32) terms takes a 256 x 256 tile 1.25 (fp32 7.6), a 128 x 128 tile alone on its compute unit
@@ -620,7 +627,7 @@ Plan plan(int form, int type, int M, int N, int K) {
 }  // namespace
 
 int gated_splits(int form, int type, int M, int N, int K) {
-  if (form == GATED_FWD && M <= kFewRows) return 1;
+  if (form == GATED_FWD && few_rows(type, M, N, K)) return 1;
   return plan(form, type, M, N, K).splits;
 }
 
@@ -629,7 +636,7 @@ int64_t gated_part_floats(int form, int M, int N) {
 }
 
 void gated_launch(int form, int type, bool out_f32, const GatedArgs& a, hipStream_t st) {
-  if (form == GATED_FWD && a.M <= kFewRows) {
+  if (form == GATED_FWD && few_rows(type, a.M, a.N, a.K)) {
     pick_type(type, [&](auto ev) {
       using E = decltype(ev);
       const dim3 grid((uint32_t)cdiv(a.N, 16));
