@@ -132,7 +132,9 @@ __device__ __forceinline__ void store4(O* row, int n, int N, const f32x4& v, boo
 
 // ---------------------------------------------------------------------------- tiled product
 template <typename E, typename O, int FORM, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM* WN * 64) void gated_kernel(GatedArgs a, int mt, int nt) {
+// (two waves a SIMD is what the LDS leaves room for: told so, the compiler keeps the sums out of AGPRs)
+__global__ __launch_bounds__(WM* WN * 64)
+__attribute__((amdgpu_waves_per_eu(2, 2))) void gated_kernel(GatedArgs a, int mt, int nt) {
   constexpr int NW = WM * WN, NT = NW * 64;
   constexpr int TM = BM / WM, TN = BN / WN;          // a wave's tile
   constexpr int MF = TM / 16, NF = TN / 16;
