@@ -3,7 +3,8 @@
 
 Reference flags: --lr (0.1), --resume/-r. Additive flags: --model (default SimpleDLA, the
 reference's main.py:71 choice), --epochs (200), --batch_size (128), --test_batch_size (100),
---data_dir, --synthetic, --seed, --graph, --max_steps, --log_every, --checkpoint_dir, --cpu.
+--data_dir, --synthetic, --seed, --graph, --max_steps, --log_every, --checkpoint_dir, --cpu,
+--teacher / --teacher_ckpt / --distill_* (learn from another zoo model's answers).
 
 Semantics kept: RandomCrop(32, pad 4) + HFlip + Normalize train transform, SGD(momentum 0.9,
 wd 5e-4), CosineAnnealingLR(T_max=200) stepped per epoch, CE loss, best-accuracy checkpoint
@@ -17,6 +18,7 @@ import torch
 
 from pytorch_cifar_amd import models
 from pytorch_cifar_amd.data.factory import build_loaders
+from pytorch_cifar_amd.engine import distillation
 from pytorch_cifar_amd.engine.arena import ParamArena
 from pytorch_cifar_amd.engine.checkpoint import load_checkpoint, save_checkpoint
 from pytorch_cifar_amd.engine.optim import SGD
@@ -56,6 +58,7 @@ parser.add_argument('--nproc', default=None, type=int,
                     help='data-parallel ranks (default: every visible GPU, one process each; '
                          'the reference main.py:74 DataParallel used all GPUs too)')
 parser.add_argument('--bucket_mb', default=4.0, type=float, help='gradient all-reduce bucket size (MiB)')
+distillation.add_arguments(parser)
 
 
 
@@ -107,6 +110,7 @@ def _data_parallel_ranks(args):
 
 def main(argv=None):
     args = parser.parse_args(argv)
+    distillation.check_arguments(parser, args)
     nranks = _data_parallel_ranks(args)
     if nranks > 1 and launcher.spawned_world() == 0:
         # Reference main.py:73-74 wraps the net in nn.DataParallel over every visible GPU. Here each
@@ -167,7 +171,8 @@ def main(argv=None):
     trainer = Trainer(net, optimizer, trainloader, testloader, ctx, ddp=ddp,
                       graph=bool(args.graph) and device.type == 'cuda', log_every=args.log_every,
                       progress=progress_bar if is_main else None, max_steps=args.max_steps,
-                      nan_guard=not args.no_nan_guard, is_main=is_main)
+                      nan_guard=not args.no_nan_guard,
+                      distill=distillation.from_arguments(args, device), is_main=is_main)
     prof_cm = None
     if args.profile and is_main:
         from pytorch_cifar_amd.utils.profiling import torch_profile

@@ -4,7 +4,8 @@
 Reference flags (main_dist.py:25-46): --lr 0.1, --batch_size 512 (global), --epochs 100,
 --output_dir (required), --resume/-r, --workers 4, --world_size -1, --rank -1, --dist_url,
 --dist, --amp. Additive: --model (default ResNet152 as main_dist.py:136), --t_max (200),
---data_dir, --synthetic, --seed, --graph, --max_steps, --bucket_mb, --log_every, --no_broadcast_buffers.
+--data_dir, --synthetic, --seed, --graph, --max_steps, --bucket_mb, --log_every, --no_broadcast_buffers,
+--teacher / --teacher_ckpt / --distill_* (learn from another zoo model's answers).
 
 Launch modes:
   torchrun --nproc-per-node N main_dist.py ...      one process per GPU (RANK/WORLD_SIZE env)
@@ -29,6 +30,7 @@ import torch.multiprocessing as mp
 
 from pytorch_cifar_amd import models
 from pytorch_cifar_amd.data.factory import build_loaders
+from pytorch_cifar_amd.engine import distillation
 from pytorch_cifar_amd.engine.arena import ParamArena
 from pytorch_cifar_amd.engine.checkpoint import load_checkpoint, save_checkpoint
 from pytorch_cifar_amd.engine.optim import SGD
@@ -77,6 +79,7 @@ parser.add_argument('--debug_sync', action='store_true',
 parser.add_argument('--profile', default=None, metavar='TRACE.json',
                     help='torch.profiler Chrome trace of the first training steps')
 parser.add_argument('--no_nan_guard', action='store_true', help='do not stop on a non-finite loss')
+distillation.add_arguments(parser)
 
 best_acc = 0
 
@@ -101,6 +104,7 @@ def _apply_runtime_flags(args, loaders):
 
 def main(argv=None):
     args = parser.parse_args(argv)
+    distillation.check_arguments(parser, args)
     if launcher.spawned_world() > 1 and not args.dist:
         ctx = launcher.init_from_env(backend='gloo' if args.cpu else 'nccl')
         return main_worker(ctx, args)
@@ -191,7 +195,8 @@ def main_worker(ctx, args):
         tqdm_progress = progress_bar
     trainer = Trainer(net, optimizer, trainloader, testloader, ctx, ddp=ddp,
                       graph=bool(args.graph) and device.type == 'cuda', log_every=args.log_every,
-                      progress=tqdm_progress, max_steps=args.max_steps, nan_guard=not args.no_nan_guard)
+                      progress=tqdm_progress, max_steps=args.max_steps, nan_guard=not args.no_nan_guard,
+                      distill=distillation.from_arguments(args, device))
     prof_cm = None
     if args.profile and ctx.rank == 0:
         from pytorch_cifar_amd.utils.profiling import torch_profile

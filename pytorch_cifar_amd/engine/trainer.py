@@ -28,8 +28,9 @@ class NonFiniteLossError(FloatingPointError):
 
 class TrainStep:
     def __init__(self, net, optimizer, loader, batch_size, ddp=None, graph=False, metrics=None,
-                 clear_grads_in_step=None):
+                 clear_grads_in_step=None, distill=None):
         self.net = net
+        self.distill = distill       # engine.distillation.Distillation: a teacher beside the labels
         self.opt = optimizer
         self.loader = loader
         self.B = batch_size
@@ -78,8 +79,12 @@ class TrainStep:
             self.opt.zero_grad()
         self._grads_clean = False
         with trace_range("forward"):
-            out = self.net(x)
-            loss = cross_entropy(out, y, self.metrics)
+            if self.distill is None:
+                out = self.net(x)
+                loss = cross_entropy(out, y, self.metrics)
+            else:
+                top = self.distill.answer(x)
+                loss = self.distill.loss(self.net(x), top, y, self.metrics)
         with trace_range("backward"):
             loss.backward(unit_grad(loss))
             if self.ddp is not None:
@@ -335,7 +340,7 @@ class Trainer:
 
     def __init__(self, net, optimizer, train_loader, test_loader, ctx, ddp=None, graph=False,
                  log_every=20, progress=None, is_main=True, max_steps=None, nan_guard=True,
-                 profiler=None):
+                 profiler=None, distill=None):
         self.net = net
         self.opt = optimizer
         self.train_loader = train_loader
@@ -348,7 +353,7 @@ class Trainer:
         self.is_main = is_main
         self.max_steps = max_steps
         self.step = TrainStep(net, optimizer, train_loader, train_loader.batch_size, ddp=ddp,
-                              graph=graph)
+                              graph=graph, distill=distill)
         self.images_per_sec = None
         self.nan_guard = nan_guard
         self.profiler = profiler   # torch.profiler session stepped once per train step
