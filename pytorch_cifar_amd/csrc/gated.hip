@@ -209,6 +209,10 @@ __attribute__((amdgpu_waves_per_eu(2, 2))) void gated_kernel(GatedArgs a, int mt
   if constexpr (kTermsQ) qb += ((int64_t)half * a.qseg + m0) * ES;
   else qb += (int64_t)m0 * a.ldq * ES;
 
+  // (held in registers: picked from the arguments in the loop, the pointer would be loaded, and waited
+  // for with all LDS reads, at every K tile)
+  const char *p0 = reinterpret_cast<const char*>(a.p0), *p1 = reinterpret_cast<const char*>(a.p1);
+  asm("" : "+s"(p0), "+s"(p1));
   // K tile t: its first term and where it lies
   struct Src {
     int k0;
@@ -220,8 +224,8 @@ __attribute__((amdgpu_waves_per_eu(2, 2))) void gated_kernel(GatedArgs a, int mt
     s.k0 = (t - (seg ? per_seg : 0)) * BK;
     s.q = qb + (kTermsQ ? (int64_t)s.k0 * a.ldq : (int64_t)s.k0 + seg * a.qseg) * ES;
     const int64_t at = (kFwd ? (int64_t)n0 * a.ldp + s.k0 : (int64_t)s.k0 * a.ldp + n0) * ES;
-    s.p = reinterpret_cast<const char*>(seg ? a.p1 : a.p0) + at;
-    s.u = reinterpret_cast<const char*>(a.p1) + at;   // (forward: the other weight)
+    s.p = (seg ? p1 : p0) + at;
+    s.u = p1 + at;   // (forward: the other weight)
     return s;
   };
   constexpr int kPieces = QP + PP;
