@@ -50,6 +50,36 @@ struct Mat<float> {
   }
 };
 
+// fp32 products on the bf16 matrix instruction. A float is the exact sum of three bf16, its 8 leading
+// bits, the next 8 and the last (cut off, not rounded: 8 bits each), and of the nine products of two
+// such sums the six largest are taken: what is left out is 2^-23 of a product at most. Six
+// instructions of 32 terms take 96 cycles, the eight fp32 ones 256: gated_linear of 1021 x 512 -> 1365
+// forward and backward 127 -> 103 us; 2048 x 2048 -> 5504
+// forward at 190 TFLOP/s, the library's fp32 product at 140. (Below 2^-110 the last parts leave the type's range.) An
+// infinity has no such parts: a tile that meets one is computed again by the fp32 instruction.
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+struct Split {
+  bf16x8 h, m, l;
+};
+__device__ __forceinline__ Split split3(const f32x8& v) {
+  uint32_t a[8], b[8], c[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    a[e] = __float_as_uint(v[e]);
+    const float r = v[e] - __uint_as_float(a[e] & 0xffff0000u);
+    b[e] = __float_as_uint(r);
+    c[e] = __float_as_uint(r - __uint_as_float(b[e] & 0xffff0000u));
+  }
+  auto high = [](const uint32_t* x) {   // the upper halves
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x07060302u);
+    bf16x8 o;
+    __builtin_memcpy(&o, w, 16);
+    return o;
+  };
+  return {high(a), high(b), high(c)};
+}
 constexpr int kRow = 128;   // bytes of a row that a K tile takes: 64 16-bit or 32 fp32 terms
 template <typename E>
 constexpr int kBK = kRow / (int)sizeof(E);
@@ -246,41 +276,106 @@ __attribute__((amdgpu_waves_per_eu(2, 2))) void gated_kernel(GatedArgs a, int mt
 #pragma unroll
     for (int j = 0; j < MF; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
 
-  // A K tile is two steps of 64 bytes of terms. While a step's products run, the next step's
-  // fragments are read in the place of those that are done; between the last step of a tile and the
-  // first of the next stands the tile's one barrier: all waves have read the old buffer, which the
-  // tile after next then fills, and all pieces of the next have landed.
-  typename Mat<E>::frag q[MF], p[NF];
+  // A K tile is two steps of 64 bytes of terms (fp32: one of 128). While a step's products run, the
+  // next step's fragments are read in the place of those that are done; between the last step of a
+  // tile and the first of the next stands the tile's one barrier: all waves have read the old buffer,
+  // which the tile after next then fills, and all pieces of the next have landed.
+  constexpr bool kF32 = ES == 4;
+  typedef std::conditional_t<kF32, f32x8, typename Mat<E>::frag> Frag;
+  Frag q[MF], p[NF];
+  auto fragment = [&](auto terms, const char* from, int at, int s) -> Frag {
+    auto one = [&](int s) {
+      return decltype(terms)::value ? frag_terms<E>(from, at, s, lane) : frag_rows<E>(from, at, s, lane);
+    };
+    if constexpr (kF32) return __builtin_shufflevector(one(0), one(1), 0, 1, 2, 3, 4, 5, 6, 7);
+    else return one(s);
+  };
   auto read_q = [&](int buf, int s, int j) {
-    return kTermsQ ? frag_terms<E>(lds[buf], wm * TM + 16 * j, s, lane)
-                   : frag_rows<E>(lds[buf], wm * TM + 16 * j, s, lane);
+    return fragment(std::integral_constant<bool, kTermsQ>(), lds[buf], wm * TM + 16 * j, s);
   };
   auto read_p = [&](int buf, int s, int i) {
-    return kTermsP ? frag_terms<E>(lds[buf] + QB, wn * TN + 16 * i, s, lane)
-                   : frag_rows<E>(lds[buf] + QB, wn * TN + 16 * i, s, lane);
+    return fragment(std::integral_constant<bool, kTermsP>(), lds[buf] + QB, wn * TN + 16 * i, s);
+  };
+  // fp32: the largest magnitude that the wave has read (a NaN is passed over)
+  float most = 0.f;
+  auto look = [&](const Frag& v) {
+    if constexpr (kF32) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 2)
+        asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(most) : "v"(most), "v"(v[e]), "v"(v[e + 1]));
+    }
+  };
+  // products of q[j]; `between(j)` follows those of each
+  auto products = [&](auto between) {
+    if constexpr (!kF32) {
+#pragma unroll
+      for (int j = 0; j < MF; ++j) {
+#pragma unroll
+        for (int i = 0; i < NF; ++i) Mat<E>::mma(p[i], q[j], acc[i][j]);
+        between(j);
+      }
+    } else {
+      Split ps[NF];
+#pragma unroll
+      for (int i = 0; i < NF; ++i) look(p[i]), ps[i] = split3(p[i]);
+      typedef Mat<bf16> B;
+      look(q[0]);
+      Split qs = split3(q[0]);
+#pragma unroll
+      for (int j = 0; j < MF; ++j) {
+        Split then = qs;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < NF; ++i) B::mma(ps[i].l, qs.h, acc[i][j]);
+#pragma unroll
+        for (int i = 0; i < NF; ++i) B::mma(ps[i].h, qs.l, acc[i][j]);
+#pragma unroll
+        for (int i = 0; i < NF; ++i) B::mma(ps[i].m, qs.m, acc[i][j]);
+#pragma unroll
+        for (int i = 0; i < NF; ++i) B::mma(ps[i].m, qs.h, acc[i][j]);
+#pragma unroll
+        for (int i = 0; i < NF; ++i) B::mma(ps[i].h, qs.m, acc[i][j]);
+#pragma unroll
+        for (int i = 0; i < NF; ++i) B::mma(ps[i].h, qs.h, acc[i][j]);
+        if (j + 1 < MF) {   // the next fragment's parts between them
+          look(q[j + 1]);
+          then = split3(q[j + 1]);
+        }
+#pragma unroll
+        for (int k = 0; k < 6 * NF; ++k) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x2, 3, 0);
+        }
+        qs = then;
+        between(j);
+      }
+    }
   };
   // The step's products on q, p, the reads of the next behind the first of them (by the step's end
   // they have long arrived), and, with `src`, the pieces of a later tile between them: issued all at
   // once they would hold the products up until the last wave's have been taken.
   auto step = [&](auto fill, int buf, int s, const Src& src, int to) {
-    typename Mat<E>::frag nq[MF], np[NF];
+    Frag nq[MF], np[NF];
     constexpr int kG = MF >= 4 ? MF / 2 : 1, kFrags = (NF + MF + kG - 1) / kG;
     constexpr int kEach = (kPieces + MF - 1) / MF;
+    products([&](int j) {
+      if constexpr (kF32) {   // (each in the registers of one that is done with)
+        nq[j] = read_q(buf, s, j);
 #pragma unroll
-    for (int j = 0; j < MF; ++j) {
+        for (int i = j; i < NF; i += MF) np[i] = read_p(buf, s, i);
+      } else {
 #pragma unroll
-      for (int i = 0; i < NF; ++i) Mat<E>::mma(p[i], q[j], acc[i][j]);
-#pragma unroll
-      for (int r = j * kFrags; r < (j + 1) * kFrags; ++r) {
-        if (r < NF) np[r] = read_p(buf, s, r);
-        else if (r < NF + MF) nq[r - NF] = read_q(buf, s, r - NF);
+        for (int r = j * kFrags; r < (j + 1) * kFrags; ++r) {
+          if (r < NF) np[r] = read_p(buf, s, r);
+          else if (r < NF + MF) nq[r - NF] = read_q(buf, s, r - NF);
+        }
       }
       if constexpr (decltype(fill)::value) {
 #pragma unroll
         for (int i = j * kEach; i < (j + 1) * kEach && i < kPieces; ++i) issue(src, to, i);
       }
-      __builtin_amdgcn_sched_barrier(0);
-    }
+      if constexpr (!kF32) __builtin_amdgcn_sched_barrier(0);
+    });
 #pragma unroll
     for (int i = 0; i < NF; ++i) p[i] = np[i];
 #pragma unroll
@@ -316,23 +411,53 @@ __attribute__((amdgpu_waves_per_eu(2, 2))) void gated_kernel(GatedArgs a, int mt
   for (; t + 2 < t1; ++t) {
     const int buf = (t - t0) & 1;
     const Src src = source(t + 2);
-    step(kNoFill, buf, 1, src, 0);
+    if constexpr (!kF32) step(kNoFill, buf, 1, src, 0);
     turn();
     step(kFill, buf ^ 1, 0, src, buf);
   }
   if (t + 1 < t1) {
     const int buf = (t - t0) & 1;
-    step(kNoFill, buf, 1, Src(), 0);
+    if constexpr (!kF32) step(kNoFill, buf, 1, Src(), 0);
     turn();
     step(kNoFill, buf ^ 1, 0, Src(), 0);
     ++t;
   }
   if (t < t1) {
-    step(kNoFill, (t - t0) & 1, 1, Src(), 0);
+    if constexpr (!kF32) step(kNoFill, (t - t0) & 1, 1, Src(), 0);
+    products([](int) {});
+  }
+  if constexpr (kF32) {
+    int* met = reinterpret_cast<int*>(&lds[0][0]);
+    __syncthreads();
+    if (threadIdx.x == 0) *met = 0;
+    __syncthreads();
+    if (most == INFINITY) *met = 1;
+    __syncthreads();
+    const bool again = *met != 0;
+    __syncthreads();
+    if (again) {
 #pragma unroll
-    for (int j = 0; j < MF; ++j)
+      for (int i = 0; i < NF; ++i)
 #pragma unroll
-      for (int i = 0; i < NF; ++i) Mat<E>::mma(p[i], q[j], acc[i][j]);
+        for (int j = 0; j < MF; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
+      for (int t = t0; t < t1; ++t) {
+        const Src src = source(t);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) issue(src, 0, i);
+        turn();
+#pragma unroll
+        for (int j = 0; j < MF; ++j) {
+          const Frag x = read_q(0, 0, j);
+#pragma unroll
+          for (int i = 0; i < NF; ++i) {
+            const Frag y = read_p(0, 0, i);
+            Mat<float>::mma(__builtin_shufflevector(y, y, 0, 1, 2, 3), __builtin_shufflevector(x, x, 0, 1, 2, 3), acc[i][j]);
+            Mat<float>::mma(__builtin_shufflevector(y, y, 4, 5, 6, 7), __builtin_shufflevector(x, x, 4, 5, 6, 7), acc[i][j]);
+          }
+        }
+        turn();
+      }
+    }
   }
 
   // ---- epilogue: lane holds columns 4 (lane >> 4) .. + 3 of row (lane & 15) of each 16 x 16 tile
@@ -599,9 +724,10 @@ bool few_rows(int type, int M, int N, int K) {
 }
 
 // Tiles and splits of the sum by a model of the time in us, from measured times: a K tile of 64
-// (fp32: 32) terms takes a 256 x 256 tile 1.25 (fp32 7.6), a 128 x 128 tile alone on its compute unit
-// 0.65 (2.1) and two that share one 1.11 (3.9); a tile's start and end take 12 and 8; the partial sums
-// of splits are written and read at 4.5 TB/s by one more launch.
+// (fp32: 32) terms takes a 256 x 256 tile 1.25, a 128 x 128 tile alone on its compute unit 0.65 (fp32
+// 1.5) and two that share one 1.11 (2.5); a tile's start and end take 12 and 8; the partial sums of
+// splits are written and read at 4.5 TB/s by one more launch. (dx of 4096 x 2048 <- 5504 bf16, 128 large
+// tiles: in small tiles 201 us, in two splits 162 + 16.)
 struct Plan {
   bool big;
   int mt, nt, splits;
@@ -612,12 +738,12 @@ Plan plan(int form, int type, int M, int N, int K) {
   const int nk = (form == GATED_DX ? 2 : 1) * cdiv(K, kRow / (f32 ? 4 : 2));
   Plan best{};
   double least = 0;
-  for (int big = 0; big < 2; ++big) {
+  for (int big = 0; big < (f32 ? 1 : 2); ++big) {
     const int b = big ? 256 : 128;
     const int mt = halves * cdiv(M, b), nt = cdiv(N * nh, b);
     for (int s = 1; s <= 16 && (s == 1 || nk / s >= 4); ++s) {
       const int64_t n = (int64_t)mt * nt * s;
-      const double each = big ? (f32 ? 7.6 : 1.25) : n <= kCUs ? (f32 ? 2.1 : 0.65) : f32 ? 3.9 : 1.11;
+      const double each = big ? 1.25 : n <= kCUs ? (f32 ? 1.5 : 0.65) : f32 ? 2.5 : 1.11;
       const double rounds = (double)cdiv64(n, big || n <= kCUs ? kCUs : 2 * kCUs);
       double us = rounds * (cdiv(nk, s) * each + (big ? 12 : 8));
       if (s > 1) us += 5 + (double)M * N * halves * nh * 4 * (2 * s) / 4.5e6;
@@ -660,9 +786,10 @@ void gated_launch(int form, int type, bool out_f32, const GatedArgs& a, hipStrea
     using E = decltype(ev);
     using O = decltype(ov);
     constexpr int FORM = decltype(fv)::value;
-    if (p.big)
-      hipLaunchKernelGGL((gated_kernel<E, O, FORM, 256, 256, 2, 4>), grid, dim3(512), 0, st, a, p.mt, p.nt);
-    else
+    if (p.big) {
+      if constexpr (sizeof(E) == 2)   // (fp32: its fragments take the registers of 128 x 128)
+        hipLaunchKernelGGL((gated_kernel<E, O, FORM, 256, 256, 2, 4>), grid, dim3(512), 0, st, a, p.mt, p.nt);
+    } else
       hipLaunchKernelGGL((gated_kernel<E, O, FORM, 128, 128, 2, 2>), grid, dim3(256), 0, st, a, p.mt, p.nt);
     if (a.part)
       hipLaunchKernelGGL((gated_join_kernel<O, FORM>), dim3(grid_for(n)), dim3(256), 0, st, a, n);
