@@ -2,6 +2,7 @@
 // current stream of the tensors' own device (no host sync, hipGraph-capturable). The loss's autograd
 // node is C++: at the sizes of a CIFAR batch the step is bound by the host.
 #include <cmath>
+#include <mutex>
 
 #include "bindings_util.h"
 #include "distill.h"
@@ -214,16 +215,21 @@ Tensor distill_loss(const Tensor& logits, const Tensor& values, const Tensor& in
   return l.reduction == 0 && logits.dim() != 2 ? loss.view(rows) : loss;
 }
 
-// never destroyed: their memory may outlive the allocator at exit
-std::vector<Tensor>& units() {
-  static auto* u = new std::vector<Tensor>();
+// never destroyed: their memory may outlive the allocator at exit. (Read by autograd's threads.)
+struct Units {
+  std::mutex lock;
+  std::vector<Tensor> t;
+};
+Units& units() {
+  static auto* u = new Units();
   return *u;
 }
 
 }  // namespace
 
 bool is_unit_seed(const Tensor& g) {
-  for (const Tensor& u : units())
+  std::lock_guard<std::mutex> hold(units().lock);
+  for (const Tensor& u : units().t)
     if (u.data_ptr() == g.data_ptr() && u.sizes() == g.sizes() &&
         u.scalar_type() == g.scalar_type())
       return true;
@@ -237,7 +243,10 @@ void register_distill(py::module& m) {
         py::arg("lse"), py::arg("target"), py::arg("temperature"), py::arg("alpha"),
         py::arg("tail"), py::arg("reduction"), py::arg("ignore_index"), py::arg("debug"),
         "differentiable loss against a teacher's top logits");
-  m.def("register_unit_seed", [](const Tensor& t) { units().push_back(t); },
+  m.def("register_unit_seed", [](const Tensor& t) {
+    std::lock_guard<std::mutex> hold(units().lock);
+    units().t.push_back(t);
+  },
         "a tensor of ones that is never written: backward passes seeded with it scale nothing");
 }
 

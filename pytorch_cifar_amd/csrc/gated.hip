@@ -131,7 +131,7 @@ __device__ __forceinline__ float sigmoid(float x) {
 __device__ __forceinline__ float act_val(float g, int act) {
   if (act == ACT_SWISH) return g * sigmoid(g);
   if (act == ACT_SIGMOID) return sigmoid(g);
-  return act == ACT_RELU ? fmaxf(g, 0.f) : g;
+  return act == ACT_RELU && g < 0.f ? 0.f : g;   // (a NaN stays one)
 }
 // act(g) and its slope
 __device__ __forceinline__ void act_both(float g, int act, float& v, float& slope) {
@@ -140,8 +140,8 @@ __device__ __forceinline__ void act_both(float g, int act, float& v, float& slop
     v = act == ACT_SWISH ? g * s : s;
     slope = act == ACT_SWISH ? fmaf(v, 1.f - s, s) : s * (1.f - s);
   } else {
-    v = act == ACT_RELU ? fmaxf(g, 0.f) : g;
-    slope = act == ACT_RELU && !(g > 0.f) ? 0.f : 1.f;
+    v = act == ACT_RELU && g < 0.f ? 0.f : g;
+    slope = act == ACT_RELU && g <= 0.f ? 0.f : 1.f;
   }
 }
 

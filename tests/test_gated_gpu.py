@@ -228,6 +228,26 @@ def test_values_stay_in_their_rows():
     assert torch.equal(h[:, cols], base[0][:, cols]) and torch.equal(dwg[cols], base[2][cols])
 
 
+@pytest.mark.parametrize("act", ["swish", "relu", None])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinities_are_those_of_the_formula(dtype, act):
+    """One infinity in a row, one in a weight, a NaN in another: the same infinities and NaN as the
+    formula's, and finite values where it has them. (The rows are few enough for one sum a unit.)"""
+    for m in (5, 300):
+        x, wg, wu, dh = inputs(m, 64, 136, dtype, 7)
+        x[3, 9] = float("inf")
+        wg[20, 4] = -float("inf")
+        wu[30, 5] = float("nan")
+        wg[:, 9] = wg[:, 9].float().abs().clamp_min(2.0 ** -6).to(dtype)   # (a product of 1 and of 8 bits each)
+        h = PF.gated_linear(x, wg, wu, act)
+        g, u = x.double() @ wg.double().t(), x.double() @ wu.double().t()
+        want = {"swish": g * torch.sigmoid(g), "relu": torch.relu(g), None: g}[act] * u
+        want = torch.where(g.isnan(), g, want)
+        assert torch.equal(h.isnan(), want.isnan())
+        assert torch.equal(h.double()[want.isinf()], want[want.isinf()])
+        assert torch.isfinite(h[torch.isfinite(want)]).all()
+
+
 def test_other_stream_and_same_bits():
     x, wg, wu, dh = inputs(100, 520, 2100, torch.bfloat16, 8)
     first = run(x, wg, wu, dh, "swish")
