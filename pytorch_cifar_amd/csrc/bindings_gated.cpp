@@ -59,7 +59,7 @@ std::pair<Tensor, Tensor> weights(const Tensor& wg, const Tensor& wu, at::Scalar
 
 void run(int form, const Tensor& like, bool out_f32, GatedArgs& a) {
   const int type = gated_type(like);
-  a.splits = gated_splits(form, type, a.M, a.N, a.K);
+  a.splits = gated_splits(form, type, a.M, a.N, a.K, std::max(a.parts, 1));
   Tensor part;
   if (a.splits > 1) {
     part = at::empty({a.splits * gated_part_floats(form, a.M, a.N)},
@@ -114,11 +114,12 @@ std::tuple<Tensor, Tensor, Tensor> backward(const Tensor& dh, const Tensor& x, c
     }
     return {dx, dwg, dwu};
   }
-  auto d = at::empty({M, 2 * Fp}, x.options());
+  const int parts = gated_parts(gated_type(x), M, C, F);
+  auto d = at::empty({M, 2 * parts * Fp}, x.options());
   gated_dact_launch(gated_type(x), g.data_ptr<float>(), u.data_ptr<float>(), dh.data_ptr(),
-                    dh.stride(0), M, (int)F, (int)Fp, act, d.data_ptr(), cur_stream());
+                    dh.stride(0), M, (int)F, (int)Fp, act, parts, d.data_ptr(), cur_stream());
   GatedArgs a{};
-  a.q = d.data_ptr(), a.ldq = 2 * Fp, a.qseg = Fp;
+  a.q = d.data_ptr(), a.ldq = 2 * parts * Fp, a.qseg = Fp, a.parts = parts;
   a.N = (int)C, a.ncols = (int)Cp;
   if (need_dx) {
     GatedArgs b = a;
@@ -194,7 +195,7 @@ Tensor gated_linear(const Tensor& x, const Tensor& wg, const Tensor& wu, int64_t
            wu.scalar_type());
   PCA_VALUE(wg.device() == x.device() && wu.device() == x.device(), "weights are on ", wg.device(),
             " and ", wu.device(), ", x is on ", x.device());
-  PCA_VALUE(x.numel() / x.size(-1) < (int64_t(1) << 31), "x has too many rows");
+  PCA_VALUE(x.numel() / x.size(-1) <= (int64_t(1) << 30), "x has more than 2^30 rows");
   PCA_VALUE(act >= ACT_NONE && act <= ACT_SIGMOID, "activation");
   c10::OptionalDeviceGuard guard(at::device_of(x));
   Tensor h;

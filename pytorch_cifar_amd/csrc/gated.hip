@@ -7,7 +7,7 @@
 //   dX       [dg | du] times [Wg; Wu], one sum over both halves;
 //   dW       [dg | du]^T x.
 // dg = dh u act'(g) and du = dh act(g) are formed from the fp32 projections and rounded once to the
-// operands' type.
+// operands' type; in small products, which do not average the roundings out, in two parts.
 #include "gated.h"
 #include "mfma_util.h"
 
@@ -193,7 +193,7 @@ __attribute__((amdgpu_waves_per_eu(2, 2))) void gated_kernel(GatedArgs a, int mt
   const int m0 = mi * BM, n0 = ni * NH;
 
   const int per_seg = (a.K + BK - 1) / BK;
-  const int nk = FORM == GATED_DX ? 2 * per_seg : per_seg;
+  const int nk = (FORM == GATED_DX ? 2 * a.parts : FORM == GATED_DW ? a.parts : 1) * per_seg;
   const int split = blockIdx.y;
   const int t0 = (int)((int64_t)nk * split / gridDim.y);
   const int t1 = (int)((int64_t)nk * (split + 1) / gridDim.y);
@@ -249,12 +249,13 @@ __attribute__((amdgpu_waves_per_eu(2, 2))) void gated_kernel(GatedArgs a, int mt
     const char *q, *p, *u;
   };
   auto source = [&](int t) {
-    const int seg = FORM == GATED_DX && t >= per_seg;
+    int seg = 0;
+    if constexpr (!kFwd) seg = (t >= per_seg) + (t >= 2 * per_seg) + (t >= 3 * per_seg);
     Src s;
-    s.k0 = (t - (seg ? per_seg : 0)) * BK;
-    s.q = qb + (kTermsQ ? (int64_t)s.k0 * a.ldq : (int64_t)s.k0 + seg * a.qseg) * ES;
+    s.k0 = (t - seg * per_seg) * BK;
+    s.q = qb + (kTermsQ ? (int64_t)s.k0 * a.ldq + 2 * seg * a.qseg : (int64_t)s.k0 + seg * a.qseg) * ES;
     const int64_t at = (kFwd ? (int64_t)n0 * a.ldp + s.k0 : (int64_t)s.k0 * a.ldp + n0) * ES;
-    s.p = (seg ? p1 : p0) + at;
+    s.p = (FORM == GATED_DX && (seg & 1) ? p1 : p0) + at;
     s.u = p1 + at;   // (forward: the other weight)
     return s;
   };
@@ -644,13 +645,13 @@ __global__ __launch_bounds__(256) void gated_dact_kernel(const float* __restrict
                                                          const float* __restrict__ u,
                                                          const E* __restrict__ dh, int64_t lddh,
                                                          int64_t M, int F, int Fp, int act,
-                                                         E* __restrict__ out) {
+                                                         int parts, E* __restrict__ out) {
   constexpr int PC = kPiece<E>;
   const int pieces = Fp / PC;
   for (int64_t w = blockIdx.x * 256ll + threadIdx.x; w < M * pieces; w += (int64_t)gridDim.x * 256) {
     const int64_t m = w / pieces;
     const int f0 = (int)(w % pieces) * PC;
-    E dg[PC], du[PC];
+    E dg[PC], du[PC], dg2[PC], du2[PC];
     float gv[PC], uv[PC];
     E d[PC];
     if (f0 + PC <= F) {
@@ -671,12 +672,20 @@ __global__ __launch_bounds__(256) void gated_dact_kernel(const float* __restrict
       const float df = static_cast<float>(d[i]);
       float v, slope;
       act_both(gv[i], act, v, slope);
-      dg[i] = static_cast<E>(df * uv[i] * slope);
-      du[i] = static_cast<E>(df * v);
+      const float a = df * uv[i] * slope, b = df * v;
+      dg[i] = static_cast<E>(a);
+      du[i] = static_cast<E>(b);
+      // (of an infinity nothing is left)
+      dg2[i] = static_cast<E>(isinf(static_cast<float>(dg[i])) ? 0.f : a - static_cast<float>(dg[i]));
+      du2[i] = static_cast<E>(isinf(static_cast<float>(du[i])) ? 0.f : b - static_cast<float>(du[i]));
     }
-    E* row = out + m * 2 * Fp + f0;
+    E* row = out + m * 2 * parts * Fp + f0;
     __builtin_memcpy(row, dg, 16);
     __builtin_memcpy(row + Fp, du, 16);
+    if (parts == 2) {
+      __builtin_memcpy(row + 2 * Fp, dg2, 16);
+      __builtin_memcpy(row + 3 * Fp, du2, 16);
+    }
   }
 }
 
@@ -732,10 +741,10 @@ struct Plan {
   bool big;
   int mt, nt, splits;
 };
-Plan plan(int form, int type, int M, int N, int K) {
+Plan plan(int form, int type, int M, int N, int K, int parts) {
   const int halves = form == GATED_DW ? 2 : 1, nh = form == GATED_FWD ? 2 : 1;
   const bool f32 = type == GATED_F32;
-  const int nk = (form == GATED_DX ? 2 : 1) * cdiv(K, kRow / (f32 ? 4 : 2));
+  const int nk = (form == GATED_DX ? 2 : 1) * parts * cdiv(K, kRow / (f32 ? 4 : 2));
   Plan best{};
   double least = 0;
   for (int big = 0; big < (f32 ? 1 : 2); ++big) {
@@ -758,9 +767,17 @@ Plan plan(int form, int type, int M, int N, int K) {
 
 }  // namespace
 
-int gated_splits(int form, int type, int M, int N, int K) {
+int gated_parts(int type, int64_t M, int64_t C, int64_t F) {
+  // One part's rounding is that of the result again, sqrt(2) of it together where many terms average
+  // it out; up to 1.7 was seen in gradients of a few rows, and none above 1.5 in two parts. Twice the
+  // terms are 8 M C F more operations: 256 x 512 -> 1536 backward 33 -> 34.5 us, at the bound 3 us of
+  // some 40.
+  return type != GATED_F32 && M * C * F <= 250000000 ? 2 : 1;
+}
+
+int gated_splits(int form, int type, int M, int N, int K, int parts) {
   if (form == GATED_FWD && few_rows(type, M, N, K)) return 1;
-  return plan(form, type, M, N, K).splits;
+  return plan(form, type, M, N, K, parts).splits;
 }
 
 int64_t gated_part_floats(int form, int M, int N) {
@@ -779,7 +796,7 @@ void gated_launch(int form, int type, bool out_f32, const GatedArgs& a, hipStrea
     });
     return;
   }
-  const Plan p = plan(form, type, a.M, a.N, a.K);
+  const Plan p = plan(form, type, a.M, a.N, a.K, std::max(a.parts, 1));
   const dim3 grid((uint32_t)(p.mt * p.nt), (uint32_t)a.splits);
   const int64_t n = (int64_t)a.M * a.N;
   auto go = [&](auto ev, auto ov, auto fv) {
@@ -805,11 +822,11 @@ void gated_launch(int form, int type, bool out_f32, const GatedArgs& a, hipStrea
 }
 
 void gated_dact_launch(int type, const float* g, const float* u, const void* dh, int64_t lddh,
-                       int64_t M, int F, int Fp, int act, void* dgdu, hipStream_t st) {
+                       int64_t M, int F, int Fp, int act, int parts, void* dgdu, hipStream_t st) {
   pick_type(type, [&](auto ev) {
     using E = decltype(ev);
     hipLaunchKernelGGL((gated_dact_kernel<E>), dim3(grid_for(M * (Fp / kPiece<E>))), dim3(256), 0,
-                       st, g, u, reinterpret_cast<const E*>(dh), lddh, M, F, Fp, act,
+                       st, g, u, reinterpret_cast<const E*>(dh), lddh, M, F, Fp, act, parts,
                        reinterpret_cast<E*>(dgdu));
   });
 }

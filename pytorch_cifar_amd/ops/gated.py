@@ -20,7 +20,8 @@ def gated_linear(x, w_gate, w_up, act="swish"):
     the result has ``hidden`` in the place of ``width``. ``act``: "swish" ("silu"), "sigmoid",
     "relu" or None. fp32, bf16 and fp16 rows; the weights have the rows' type, or are fp32 masters,
     which are rounded to it and whose gradients are fp32. Sums are fp32; in 16 bits the gradients of
-    the projections are rounded once to the rows' type, the operand of the products that follow.
+    the projections are rounded once to the rows' type, the operand of the products that follow (small
+    layers keep them in two parts). In fp16 what overflows there is an infinity.
     """
     if act not in ACT:
         raise ValueError(f"act must be one of {sorted(a for a in ACT if a)} or None, got {act!r}")

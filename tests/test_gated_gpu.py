@@ -300,9 +300,43 @@ def test_offsets_past_32_bits():
     # the zero rows add nothing but their places in the sums
     half = 2.0 ** -8
     want = run(tail, wg, wu, dh_tail, "swish")
-    for a, b in zip((dwg, dwu), want[2:]):
-        # two roundings of nearly the same fp32 sums: a step apart
-        assert ((a.double() - b.double()).abs() <= 2 * half * b.double().abs() + 1e-3 * b.double().abs().max()).all()
+    # The small call keeps dg and du in two parts, of error below 2^-16 of them, the large one rounds
+    # each once: its sums are off by at most half a step of every |dg_mf| |x_mc|, that is
+    # half * |dg|^T |x|, however the terms' signs fall. (1.1: fp32's share and that of the two parts.)
+    xd, gd, ud, d = (t.double() for t in (tail, wg, wu, dh_tail))
+    act, slope = act_of(xd @ gd.t(), "swish")
+    terms = [(d * (xd @ ud.t()) * slope).abs().t() @ xd.abs(), (d * act).abs().t() @ xd.abs()]
+    for a, b, e in zip((dwg, dwu), want[2:], terms):
+        # ... and two roundings of those sums: a step apart
+        assert ((a.double() - b.double()).abs() <= 1.1 * half * e
+                + 2 * half * b.double().abs() + 1e-3 * b.double().abs().max()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m, c, f", [(1, 96, 264), (2, 8, 1000), (7, 333, 40), (22, 24, 89), (200, 520, 1365)])
+def test_small_products_round_once(m, c, f, dtype):
+    """In small layers dg and du are kept in two parts: what is left of their rounding is below 2^-16
+    (bf16; fp16 2^-22, or 2^-25 where the second part is subnormal) of each, and the gradients are
+    off by half a step of themselves and the sums' share."""
+    x, wg, wu, dh = inputs(m, c, f, dtype, 12)
+    half = torch.finfo(dtype).eps / 2
+    _, *grads = run(x, wg, wu, dh, "swish")
+    xd, gd, ud, d = (t.double() for t in (x, wg, wu, dh))
+    g, u = xd @ gd.t(), xd @ ud.t()
+    a, s = act_of(g, "swish")
+    dg, du = d * u * s, d * a
+    # relative errors of dg and du: two parts, and fp32 projections (of c terms) through slopes below 1.1
+    mag = xd.abs() @ gd.abs().t(), xd.abs() @ ud.abs().t()
+    e = 1.2 * (c + 40) * U
+    near = d.abs() * (e * mag[1] * (s.abs() + 0.1) + e * mag[0] * (u.abs() + 1)) + 2.0 ** -25
+    eg, eu = (near + (half * half + 8 * U) * t.abs() for t in (dg, du))
+    want = dg @ gd + du @ ud, dg.t() @ xd, du.t() @ xd
+    off = (eg @ gd.abs() + eu @ ud.abs() + (2 * f + 2) * 2 * U * (dg.abs() @ gd.abs() + du.abs() @ ud.abs()),
+           eg.t() @ xd.abs() + (m + 2) * 2 * U * (dg.abs().t() @ xd.abs()),
+           eu.t() @ xd.abs() + (m + 2) * 2 * U * (du.abs().t() @ xd.abs()))
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    for got, w, o in zip(grads, want, off):
+        assert ((got.double() - w).abs() <= half * (w.abs() + o) + o + tiny).all()
 
 
 def test_module_trains_in_bf16():
@@ -345,6 +379,7 @@ def test_refusals_on_the_gpu():
             (ValueError, (x, wg, wu, "gelu")), (TypeError, (x.long(), wg, wu)),
             (TypeError, (x.double(), wg.double(), wu.double())), (ValueError, (x, wg[:0], wu[:0])),
             (ValueError, (z(2, 0), z(4, 0), z(4, 0))), (ValueError, (z(1, 16)[0, 0], wg, wu)),
+            (ValueError, (z(1, 1).expand((1 << 30) + 1, 1), z(4, 1), z(4, 1))),
             (ValueError, (z(1, (1 << 19) + 8), z(1, (1 << 19) + 8), z(1, (1 << 19) + 8)))]:
         with pytest.raises(err):
             PF.gated_linear(*args)
