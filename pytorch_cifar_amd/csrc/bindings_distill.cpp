@@ -110,9 +110,18 @@ std::tuple<Tensor, Tensor> distill(const Tensor& z, const Tensor& values, const 
   return {loss, dz};
 }
 
+// The capture that the current stream is in, 0: none.
+int64_t capture() {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo(cur_stream(), &status, &id) != hipSuccess) (void)hipGetLastError();
+  return status == hipStreamCaptureStatusActive ? (int64_t)id : 0;
+}
+
 // The forward computes the gradient for a unit seed from the row it holds in registers and hands it
 // to the backward, which scales it where the seed is not one. A second backward of a retained graph
-// computes it again from the saved logits.
+// computes it again from the saved logits, and so does one that is not in the forward's capture: a
+// replay of either alone would scale again what is scaled, or write over what was returned.
 struct DistillFn : public torch::autograd::Function<DistillFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& values,
                         const Tensor& indices, const optional<Tensor>& lse_,
@@ -121,6 +130,7 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
     auto [loss, dz] = distill(rows_of(logits), values, indices, lse, target, l, true);
     ctx->save_for_backward({logits, values, indices, lse, target});
     ctx->saved_data["dz"] = dz;
+    ctx->saved_data["capture"] = capture();
     ctx->saved_data["temperature"] = l.temperature;
     ctx->saved_data["alpha"] = l.alpha;
     ctx->saved_data["tail"] = l.tail;
@@ -140,7 +150,7 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
       auto& d = ctx->saved_data;
       Tensor dz;
       auto it = d.find("dz");
-      if (it != d.end()) {
+      if (it != d.end() && capture() == d["capture"].toInt()) {
         dz = it->second.toTensor();
         d.erase(it);
       } else {

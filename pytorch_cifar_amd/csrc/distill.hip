@@ -875,6 +875,13 @@ int few_rows(int64_t R, int threads) {
   return threads;
 }
 
+// A launch holds less than 2^32 threads: fn(first, rows) for each part of the R rows that one can take.
+template <typename F>
+void row_parts(int64_t R, F&& fn) {
+  constexpr int64_t kRows = 1 << 21;   // (of up to 1024 threads)
+  for (int64_t r = 0; r < R; r += kRows) fn(r, std::min(kRows, R - r));
+}
+
 template <typename F>
 void pick_type(int type, F&& fn) {
   if (type == LOGIT_F32) fn(float());
@@ -884,15 +891,19 @@ void pick_type(int type, F&& fn) {
 
 }  // namespace
 
-void top_logits_launch(const void* z, int type, int64_t ld, int64_t R, int V, int k, double temp,
-                       void* values, int32_t* indices, float* lse, hipStream_t st) {
+void top_logits_launch(const void* logits, int type, int64_t ld, int64_t R, int V, int k, double temp,
+                       void* top, int32_t* indices, float* lse, hipStream_t st) {
   const float c = (float)(1.4426950408889634 / temp);
   pick_type(type, [&](auto tv) {
     using T = decltype(tv);
+    const T* z = reinterpret_cast<const T*>(logits);
+    T* values = reinterpret_cast<T*>(top);
     if (V <= 64) {
-      hipLaunchKernelGGL((top_small_kernel<T>), dim3((uint32_t)((R + 3) / 4)), dim3(256), 0, st,
-                         reinterpret_cast<const T*>(z), ld, R, V, k, c, 1.0 / temp,
-                         reinterpret_cast<T*>(values), indices, lse);
+      row_parts(R, [&](int64_t r, int64_t rows) {
+        hipLaunchKernelGGL((top_small_kernel<T>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, st,
+                           z + r * ld, ld, rows, V, k, c, 1.0 / temp, values + r * k, indices + r * k,
+                           lse + r);
+      });
       return;
     }
     // k maxima of the threads bound the k largest while k is at most three quarters of them. Long rows:
@@ -906,9 +917,10 @@ void top_logits_launch(const void* z, int type, int64_t ld, int64_t R, int V, in
                         : few_rows(R, n <= 4096 && k <= 64 ? 256 : n <= 16384 && k <= 384 ? 512 : 1024);
     pick_row(n, threads, [&](auto block, auto nc) {
       constexpr int BLOCK = decltype(block)::value, NC = decltype(nc)::value;
-      hipLaunchKernelGGL((top_logits_kernel<T, BLOCK, NC>), dim3((uint32_t)R), dim3(BLOCK), 0, st,
-                         reinterpret_cast<const T*>(z), ld, V, k, c, 1.0 / temp,
-                         reinterpret_cast<T*>(values), indices, lse);
+      row_parts(R, [&](int64_t r, int64_t rows) {
+        hipLaunchKernelGGL((top_logits_kernel<T, BLOCK, NC>), dim3((uint32_t)rows), dim3(BLOCK), 0, st,
+                           z + r * ld, ld, V, k, c, 1.0 / temp, values + r * k, indices + r * k, lse + r);
+      });
     });
   });
 }
@@ -928,12 +940,23 @@ void distill_launch(const DistillArgs& a, hipStream_t st) {
                                                        : n <= 8192 ? 256 : 512);
     pick_row(n, threads, [&](auto block, auto nc) {
       constexpr int BLOCK = decltype(block)::value, NC = decltype(nc)::value;
-      if (a.dz)
-        hipLaunchKernelGGL((distill_kernel<T, BLOCK, NC, true>), dim3((uint32_t)a.R), dim3(BLOCK),
-                           lds, st, a, c_t);
-      else
-        hipLaunchKernelGGL((distill_kernel<T, BLOCK, NC, false>), dim3((uint32_t)a.R), dim3(BLOCK),
-                           lds, st, a, c_t);
+      row_parts(a.R, [&](int64_t r, int64_t rows) {
+        DistillArgs b = a;
+        b.R = rows;
+        b.z = reinterpret_cast<const T*>(a.z) + r * a.ld;
+        b.values = reinterpret_cast<const char*>(a.values) + r * a.K * (a.value_type == LOGIT_F32 ? 4 : 2);
+        b.indices = reinterpret_cast<const char*>(a.indices) + r * a.K * (a.index64 ? 8 : 4);
+        if (a.lse) b.lse = a.lse + r;
+        if (a.target) b.target = a.target + r;
+        if (a.dz) b.dz = reinterpret_cast<T*>(a.dz) + r * a.V;
+        b.row_loss = a.row_loss + r;
+        if (a.dz)
+          hipLaunchKernelGGL((distill_kernel<T, BLOCK, NC, true>), dim3((uint32_t)rows), dim3(BLOCK),
+                             lds, st, b, c_t);
+        else
+          hipLaunchKernelGGL((distill_kernel<T, BLOCK, NC, false>), dim3((uint32_t)rows), dim3(BLOCK),
+                             lds, st, b, c_t);
+      });
     });
   });
 }

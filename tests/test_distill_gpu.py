@@ -384,6 +384,59 @@ def test_offsets_past_32_bits():
     assert torch.equal(d[0], d[-2])
 
 
+@pytest.mark.parametrize("r, v", [((1 << 26) + 5, 2), ((1 << 21) + 3, 70)])
+def test_more_rows_than_a_launch_holds(r, v):
+    """A launch has less than 2^32 threads: rows on both sides of its parts, against small calls."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    z = torch.randn(r, v, generator=g, device="cuda", dtype=torch.bfloat16)
+    y = torch.randint(0, v, (r,), generator=g, device="cuda")
+    top = PF.top_logits(z, 1, 2.0)
+
+    def run(z, top, y):
+        x = z.detach().requires_grad_(True)
+        loss = PF.distill_loss(x, top, y, temperature=2.0, alpha=0.5, tail=True, reduction="none")
+        (d,) = torch.autograd.grad(loss, x, torch.full_like(loss, 3.0))
+        return loss.detach(), d
+
+    loss, d = run(z, top, y)
+    for at in (0, (1 << 21) - 4, r - 8):
+        rows = slice(at, at + 8)
+        t = PF.top_logits(z[rows], 1, 2.0)
+        assert all(torch.equal(a[rows], b) for a, b in zip(top, t))
+        want = run(z[rows], t, y[rows])
+        assert torch.equal(loss[rows], want[0]) and torch.equal(d[rows], want[1])
+
+
+def test_backward_in_a_graph_of_its_own():
+    """Forward and backward captured apart: replays of the backward alone, each with its own seed."""
+    z, top, y = distill_inputs(32, 1000, 20, torch.float32, 2.0)
+    z, top, y = z.cuda(), gpu_top(top), y.cuda()
+    seed = torch.ones(32, device="cuda")
+    args = dict(temperature=2.0, alpha=0.5, reduction="none")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        x = z.detach().requires_grad_(True)
+        torch.autograd.grad(PF.distill_loss(x, top, y, **args), x, seed)
+        del x
+    torch.cuda.current_stream().wait_stream(s)
+    x = z.detach().requires_grad_(True)
+    forward, backward = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(forward, stream=s):
+        loss = PF.distill_loss(x, top, y, **args)
+    with torch.cuda.graph(backward, pool=forward.pool(), stream=s):
+        (d,) = torch.autograd.grad(loss, x, seed)
+    for i in range(3):
+        forward.replay()
+        for scale in (1.0, 3.0, 0.5):
+            seed.fill_(scale)
+            backward.replay()
+            w = z.detach().requires_grad_(True)
+            (want,) = torch.autograd.grad(PF.distill_loss(w, top, y, **args), w, seed)
+            assert torch.equal(d, want)
+        z.add_(0.25 * i)
+
+
 def test_refusals_on_the_gpu():
     z, top, y = distill_inputs(4, 50, 3, torch.float32, 1.0)
     g = gpu_top(top)
