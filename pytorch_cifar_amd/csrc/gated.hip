@@ -171,7 +171,8 @@ __attribute__((amdgpu_waves_per_eu(2, 2))) void gated_kernel(GatedArgs a, int mt
   constexpr bool kFwd = FORM == GATED_FWD;
   constexpr bool kTermsQ = FORM == GATED_DW, kTermsP = FORM != GATED_FWD;
   constexpr int BK = kBK<E>, ES = sizeof(E), PC = kPiece<E>;
-  constexpr int QB = BM * kRow, PB = BN * kRow;      // bytes of a K tile
+  // bytes of a K tile (by terms: in whole blocks of columns)
+  constexpr int QB = (kTermsQ ? (BM + 127) / 128 * 128 : BM) * kRow, PB = BN * kRow;
   constexpr int QP = QB / 1024 / NW, PP = PB / 1024 / NW;   // DMA pieces of a wave
   static_assert(QB % (1024 * NW) == 0 && PB % (1024 * NW) == 0, "whole pieces a wave");
   __shared__ __attribute__((aligned(1024))) char lds[2][QB + PB];
@@ -208,7 +209,7 @@ __attribute__((amdgpu_waves_per_eu(2, 2))) void gated_kernel(GatedArgs a, int mt
       const int term = (p * 4 + (lane >> 4)) % BK, blk = p * 4 / BK;
       const int c = blk * (256 / ES) + (((lane & 15) ^ swz_terms<E>(term)) * PC);
       qk[i] = term;
-      qoff[i] = m0 + c < a.mcols ? (uint32_t)(term * a.ldq + c) * ES : kOOB;
+      qoff[i] = c < BM && m0 + c < a.mcols ? (uint32_t)(term * a.ldq + c) * ES : kOOB;
     } else {
       const int r = p * 8 + (lane >> 3), c = ((lane & 7) ^ (r & 7)) * PC;
       qk[i] = c;
@@ -243,6 +244,8 @@ __attribute__((amdgpu_waves_per_eu(2, 2))) void gated_kernel(GatedArgs a, int mt
   // for with all LDS reads, at every K tile)
   const char *p0 = reinterpret_cast<const char*>(a.p0), *p1 = reinterpret_cast<const char*>(a.p1);
   asm("" : "+s"(p0), "+s"(p1));
+  const int qseg = (int)a.qseg;
+  const bool two = a.parts == 2;
   // K tile t: its first term and where it lies
   struct Src {
     int k0;
@@ -250,10 +253,14 @@ __attribute__((amdgpu_waves_per_eu(2, 2))) void gated_kernel(GatedArgs a, int mt
   };
   auto source = [&](int t) {
     int seg = 0;
-    if constexpr (!kFwd) seg = (t >= per_seg) + (t >= 2 * per_seg) + (t >= 3 * per_seg);
+    if constexpr (FORM == GATED_DX) {
+      seg = t >= per_seg;
+      if (two) seg += (t >= 2 * per_seg) + (t >= 3 * per_seg);
+    }
+    if constexpr (FORM == GATED_DW) seg = t >= per_seg;
     Src s;
     s.k0 = (t - seg * per_seg) * BK;
-    s.q = qb + (kTermsQ ? (int64_t)s.k0 * a.ldq + 2 * seg * a.qseg : (int64_t)s.k0 + seg * a.qseg) * ES;
+    s.q = qb + (kTermsQ ? (int64_t)s.k0 * a.ldq + 2 * seg * qseg : (int64_t)(s.k0 + seg * qseg)) * ES;
     const int64_t at = (kFwd ? (int64_t)n0 * a.ldp + s.k0 : (int64_t)s.k0 * a.ldp + n0) * ES;
     s.p = (FORM == GATED_DX && (seg & 1) ? p1 : p0) + at;
     s.u = p1 + at;   // (forward: the other weight)
@@ -651,7 +658,7 @@ __global__ __launch_bounds__(256) void gated_dact_kernel(const float* __restrict
   for (int64_t w = blockIdx.x * 256ll + threadIdx.x; w < M * pieces; w += (int64_t)gridDim.x * 256) {
     const int64_t m = w / pieces;
     const int f0 = (int)(w % pieces) * PC;
-    E dg[PC], du[PC], dg2[PC], du2[PC];
+    E dg[PC], du[PC];
     float gv[PC], uv[PC];
     E d[PC];
     if (f0 + PC <= F) {
@@ -672,19 +679,23 @@ __global__ __launch_bounds__(256) void gated_dact_kernel(const float* __restrict
       const float df = static_cast<float>(d[i]);
       float v, slope;
       act_both(gv[i], act, v, slope);
-      const float a = df * uv[i] * slope, b = df * v;
-      dg[i] = static_cast<E>(a);
-      du[i] = static_cast<E>(b);
-      // (of an infinity nothing is left)
-      dg2[i] = static_cast<E>(isinf(static_cast<float>(dg[i])) ? 0.f : a - static_cast<float>(dg[i]));
-      du2[i] = static_cast<E>(isinf(static_cast<float>(du[i])) ? 0.f : b - static_cast<float>(du[i]));
+      gv[i] = df * uv[i] * slope;
+      uv[i] = df * v;
+      dg[i] = static_cast<E>(gv[i]);
+      du[i] = static_cast<E>(uv[i]);
     }
     E* row = out + m * 2 * parts * Fp + f0;
     __builtin_memcpy(row, dg, 16);
     __builtin_memcpy(row + Fp, du, 16);
-    if (parts == 2) {
-      __builtin_memcpy(row + 2 * Fp, dg2, 16);
-      __builtin_memcpy(row + 3 * Fp, du2, 16);
+    if (parts == 2) {   // (of an infinity nothing is left)
+#pragma unroll
+      for (int i = 0; i < PC; ++i) {
+        const float g0 = static_cast<float>(dg[i]), u0 = static_cast<float>(du[i]);
+        dg[i] = static_cast<E>(isinf(g0) ? 0.f : gv[i] - g0);
+        du[i] = static_cast<E>(isinf(u0) ? 0.f : uv[i] - u0);
+      }
+      __builtin_memcpy(row + 2 * Fp, dg, 16);
+      __builtin_memcpy(row + 3 * Fp, du, 16);
     }
   }
 }
@@ -733,13 +744,15 @@ bool few_rows(int type, int M, int N, int K) {
 }
 
 // Tiles and splits of the sum by a model of the time in us, from measured times: a K tile of 64
-// (fp32: 32) terms takes a 256 x 256 tile 1.25, a 128 x 128 tile alone on its compute unit 0.65 (fp32
-// 1.5) and two that share one 1.11 (2.5); a tile's start and end take 12 and 8; the partial sums of
-// splits are written and read at 4.5 TB/s by one more launch. (dx of 4096 x 2048 <- 5504 bf16, 128 large
-// tiles: in small tiles 201 us, in two splits 162 + 16.)
+// (fp32: 32) terms takes a 256 x 256 tile 1.25, a 192 x 256 tile 1.06 in the forward and 1.12 in the
+// gradients, a 128 x 128 tile alone on its compute unit 0.65 (fp32 1.5) and two that share one 1.11
+// (2.5); a tile's start and end take 12 and 8; the partial sums of splits are written and read at
+// 4.5 TB/s by one more launch. (4096 x 2048, 5504 hidden units, bf16: dx in 128 large tiles 201 us as
+// small ones, 162 + 16 in two splits; dW in 352 tiles of 256 rows, 1.4 rounds of the 256 compute
+// units, 197, in 464 of 192 rows, 1.8 rounds, 178. Forward of 4096 x 1536 -> 4224 fp16 in 528 tiles of
+// 256 rows 117, in 726 of 192 104.)
 struct Plan {
-  bool big;
-  int mt, nt, splits;
+  int bm, mt, nt, splits;
 };
 Plan plan(int form, int type, int M, int N, int K, int parts) {
   const int halves = form == GATED_DW ? 2 : 1, nh = form == GATED_FWD ? 2 : 1;
@@ -747,18 +760,18 @@ Plan plan(int form, int type, int M, int N, int K, int parts) {
   const int nk = (form == GATED_DX ? 2 : 1) * parts * cdiv(K, kRow / (f32 ? 4 : 2));
   Plan best{};
   double least = 0;
-  for (int big = 0; big < (f32 ? 1 : 2); ++big) {
-    const int b = big ? 256 : 128;
-    const int mt = halves * cdiv(M, b), nt = cdiv(N * nh, b);
+  for (int bm = 128; bm <= (f32 ? 128 : 256); bm += 64) {
+    const bool big = bm > 128;
+    const int mt = halves * cdiv(M, bm), nt = cdiv(N * nh, big ? 256 : 128);
     for (int s = 1; s <= 16 && (s == 1 || nk / s >= 4); ++s) {
       const int64_t n = (int64_t)mt * nt * s;
-      const double each = big ? 1.25 : n <= kCUs ? (f32 ? 1.5 : 0.65) : f32 ? 2.5 : 1.11;
+      const double each = bm == 256 ? 1.25 : big ? (form == GATED_FWD ? 1.06 : 1.12) : n <= kCUs ? (f32 ? 1.5 : 0.65) : f32 ? 2.5 : 1.11;
       const double rounds = (double)cdiv64(n, big || n <= kCUs ? kCUs : 2 * kCUs);
       double us = rounds * (cdiv(nk, s) * each + (big ? 12 : 8));
       if (s > 1) us += 5 + (double)M * N * halves * nh * 4 * (2 * s) / 4.5e6;
       if (least == 0 || us < least) {
         least = us;
-        best = {big != 0, mt, nt, s};
+        best = {bm, mt, nt, s};
       }
     }
   }
@@ -803,9 +816,13 @@ void gated_launch(int form, int type, bool out_f32, const GatedArgs& a, hipStrea
     using E = decltype(ev);
     using O = decltype(ov);
     constexpr int FORM = decltype(fv)::value;
-    if (p.big) {
-      if constexpr (sizeof(E) == 2)   // (fp32: its fragments take the registers of 128 x 128)
-        hipLaunchKernelGGL((gated_kernel<E, O, FORM, 256, 256, 2, 4>), grid, dim3(512), 0, st, a, p.mt, p.nt);
+    if (p.bm > 128) {
+      if constexpr (sizeof(E) == 2) {   // (fp32: its fragments take the registers of 128 x 128)
+        if (p.bm == 256)
+          hipLaunchKernelGGL((gated_kernel<E, O, FORM, 256, 256, 2, 4>), grid, dim3(512), 0, st, a, p.mt, p.nt);
+        else
+          hipLaunchKernelGGL((gated_kernel<E, O, FORM, 192, 256, 2, 4>), grid, dim3(512), 0, st, a, p.mt, p.nt);
+      }
     } else
       hipLaunchKernelGGL((gated_kernel<E, O, FORM, 128, 128, 2, 2>), grid, dim3(256), 0, st, a, p.mt, p.nt);
     if (a.part)

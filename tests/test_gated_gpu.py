@@ -23,8 +23,10 @@ DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 # rows, width, hidden
 SIZES = [(1, 8, 8), (1, 1, 1), (3, 5, 7), (2, 264, 40), (1, 1000, 333), (17, 96, 640), (130, 129, 131),
          (257, 64, 300), (64, 512, 1365), (5, 4096, 264), (300, 72, 1100)]
-# ... for which a product is run in its largest tiles: the forward, dx, dW
-LARGE = [(4100, 136, 2056), (4100, 4104, 40), (72, 2056, 4104)]
+# ... for which a product is run in tiles of 192 rows: the forward, dx, dW; of 256: the forward, dx, dW,
+# dW and dx in splits
+LARGE = [(4100, 136, 2056), (4100, 4104, 40), (72, 2056, 4104),
+         (577, 32, 8257), (6987, 1594, 32), (40, 1044, 4899), (2460, 136, 9555), (10190, 131, 2366)]
 
 
 def act_of(g, act):
