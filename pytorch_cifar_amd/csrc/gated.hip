@@ -54,9 +54,9 @@ struct Mat<float> {
 // bits, the next 8 and the last (cut off, not rounded: 8 bits each), and of the nine products of two
 // such sums the six largest are taken: what is left out is 2^-23 of a product at most. Six
 // instructions of 32 terms take 96 cycles, the eight fp32 ones 256: gated_linear of 1021 x 512 -> 1365
-// forward and backward 127 -> 103 us; 2048 x 2048 -> 5504
-// forward at 190 TFLOP/s, the library's fp32 product at 140. (Below 2^-110 the last parts leave the type's range.) An
-// infinity has no such parts: a tile that meets one is computed again by the fp32 instruction.
+// forward and backward 127 -> 104 us; 2048 x 2048 -> 5504 forward at 190 TFLOP/s, the library's fp32
+// product at 140. (Below 2^-110 the last parts leave the type's range.) An infinity has no such parts:
+// a tile that meets one is computed again by the fp32 instruction.
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 struct Split {
   bf16x8 h, m, l;
@@ -161,6 +161,10 @@ __device__ __forceinline__ void store4(O* row, int n, int N, const f32x4& v, boo
 }
 
 // ---------------------------------------------------------------------------- tiled product
+// Bound by the matrix instruction (fp32: and by the splitting before it). The wider the tile the fewer
+// LDS reads a product takes: a wave of eight has 128 x 64 sums, half of its registers. Forward of
+// 8192 x 4096 -> 10752 bf16 1044 us, 1.38 PFLOP/s (a square product of 8192 by the library 1.42); of
+// 4096 x 2048 -> 5504 175 us, 1.06 PFLOP/s: 2.7 rounds of tiles, each with 12 us at its ends.
 template <typename E, typename O, int FORM, int BM, int BN, int WM, int WN>
 // (two waves a SIMD is what the LDS leaves room for: told so, the compiler keeps the sums out of AGPRs)
 __global__ __launch_bounds__(WM* WN * 64)
@@ -525,7 +529,7 @@ __attribute__((amdgpu_waves_per_eu(2, 2))) void gated_kernel(GatedArgs a, int mt
 // Up to 64 rows: the weights are read once, straight into the fragments' registers, and that read is
 // all the time there is. A workgroup has 16 hidden units of both weights; its waves take every NW-th
 // 64 bytes of the width, and their sums are joined in LDS, in order. The rows come from the caches
-// (every workgroup reads all of them). One row, 4096 -> 10752 bf16 (176 MB): 38 us, 4.6 TB/s.
+// (every workgroup reads all of them). One row, 4096 -> 10752 bf16 (176 MB): 37 us, 4.7 TB/s.
 template <typename E, int MT, int NW>
 __global__ __launch_bounds__(NW * 64) 
 __attribute__((amdgpu_waves_per_eu(MT < 4 ? 4 : 2))) void gated_few_kernel(GatedArgs a) {
@@ -617,7 +621,8 @@ __attribute__((amdgpu_waves_per_eu(MT < 4 ? 4 : 2))) void gated_few_kernel(Gated
   }
 }
 
-// Sums of the K splits, in order, and the epilogue that follows them.
+// Sums of the K splits, in order, and the epilogue that follows them. Bound by the read of the sums:
+// two splits of 4096 x 2048 16 us.
 template <typename O, int FORM>
 __global__ __launch_bounds__(256) void gated_join_kernel(GatedArgs a, int64_t n) {
   const int64_t total = FORM == GATED_FWD || FORM == GATED_DW ? 2 * n : n;   // floats of a split
@@ -647,6 +652,7 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GatedArgs a, int64_t n)
 }
 
 // ------------------------------------------------------------------------ elementwise passes
+// dg and du. Bound by the bytes: 4096 x 5504 bf16 (316 MB) 66 us, the rate of a large copy.
 template <typename E>
 __global__ __launch_bounds__(256) void gated_dact_kernel(const float* __restrict__ g,
                                                          const float* __restrict__ u,
