@@ -239,6 +239,7 @@ __device__ __forceinline__ int key_index(uint64_t k) {
 }
 
 constexpr int kList = 2048;   // candidates that are ranked at most
+constexpr int kCount = 16;    // comparisons a thread up to which their places are counted
 // a selection may end with this many candidates: ranking them costs less than a further pass
 __device__ __forceinline__ int enough(int k) { return k + k / 2 + 64; }
 static_assert(kDistillMaxK + kDistillMaxK / 2 + 64 <= kList, "candidates fit");
@@ -294,6 +295,21 @@ __device__ uint32_t bound_of_maxima(const uint32_t* maxima, int k, int spare) { 
     else hi = mid;
   }
   return (uint32_t)lo;
+}
+
+// the wave's keys in descending order, one a lane (bitonic)
+__device__ __forceinline__ uint64_t wave_sort(uint64_t key) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int size = 2; size <= 64; size *= 2) {
+#pragma unroll
+    for (int d = size / 2; d > 0; d /= 2) {
+      const uint64_t other = __shfl_xor(key, d, 64);
+      const bool larger = ((lane & d) == 0) == ((lane & size) == 0);
+      key = (key > other) == larger ? key : other;
+    }
+  }
+  return key;
 }
 
 // One pass over the row gives each thread its maximum, its sum of exponentials, and, where the row is
@@ -472,22 +488,45 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void top_logits_kernel(
     });
     __syncthreads();
   }
-  // a candidate's place is the number of candidates before it, counted by `parts` lanes each
   const int n = (int)found;
-  int parts = 1;
-  while (parts < 64 && 2 * parts * n <= BLOCK) parts *= 2;
-  const int part_of = threadIdx.x & (parts - 1);
-  for (int i0 = 0; i0 < n; i0 += BLOCK / parts) {
-    const int i = i0 + threadIdx.x / parts;
-    const uint64_t key = i < n ? list[i] : 0;
-    int at = 0;
+  auto put = [&](uint64_t key, int at) {
+    if (at >= k) return;
+    const int idx = key_index(key);
+    values[r * k + at] = row.p[idx];
+    indices[r * k + at] = idx;
+  };
+  // A candidate's place is the number of candidates before it.
+  if (n * n <= kCount * BLOCK) {   // counted by `parts` lanes each
+    int parts = 1;
+    while (parts < 64 && 2 * parts * n <= BLOCK) parts *= 2;
+    const int part_of = threadIdx.x & (parts - 1);
+    for (int i0 = 0; i0 < n; i0 += BLOCK / parts) {
+      const int i = i0 + threadIdx.x / parts;
+      const uint64_t key = i < n ? list[i] : 0;
+      int at = 0;
 #pragma unroll 8
-    for (int j = part_of; j < n; j += parts) at += list[j] > key;
-    for (int o = 1; o < parts; o *= 2) at += __shfl_xor(at, o, 64);
-    if (i < n && at < k && part_of == 0) {
-      const int idx = key_index(key);
-      values[r * k + at] = row.p[idx];
-      indices[r * k + at] = idx;
+      for (int j = part_of; j < n; j += parts) at += list[j] > key;
+      for (int o = 1; o < parts; o *= 2) at += __shfl_xor(at, o, 64);
+      if (i < n && part_of == 0) put(key, at);
+    }
+  } else {   // in its wave's 64, which are sorted, and by search in every other 64
+    const int lane = threadIdx.x & 63, blocks = (n + 63) / 64;
+    for (int b = threadIdx.x >> 6; b < blocks; b += NW)
+      list[64 * b + lane] = wave_sort(64 * b + lane < n ? list[64 * b + lane] : 0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += BLOCK) {
+      const uint64_t key = list[i];
+      int at = i & 63;
+#pragma unroll 4
+      for (int o = 1; o < blocks; ++o) {
+        const int b = i / 64 + o;
+        const uint64_t* other = list + 64 * (b < blocks ? b : b - blocks);
+        int before = 0;
+#pragma unroll
+        for (int half = 32; half > 0; half /= 2) before += other[before + half - 1] > key ? half : 0;
+        at += before + (other[before] > key);
+      }
+      put(key, at);
     }
   }
 }
