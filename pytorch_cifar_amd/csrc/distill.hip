@@ -268,24 +268,24 @@ __device__ uint64_t bound_of_keys(const Row<T, BLOCK, NC>& row, int k, int* red)
   return lo;
 }
 
-// The same over the maxima of the row's threads (one wave, BLOCK / 64 of them a lane): at least k
-// logits are as large as the k-th largest of them, and in a row in no particular order few more.
-template <int BLOCK>
+// The same over the maxima of parts of the row (one wave, M / 64 of them a lane; 0: no such part): at
+// least k logits are as large as the k-th largest of them, and in a row in no particular order few more.
+template <int M>
 __device__ uint32_t bound_of_maxima(const uint32_t* maxima, int k, int spare) {   // at most k + spare maxima reach it, if they differ
-  constexpr int N = BLOCK / 64;
-  uint32_t v[N];
+  constexpr int N = M / 64;
+  uint32_t v[N], least = ~0u, most = 0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = maxima[threadIdx.x + i * 64];
-  uint32_t least = v[0], most = v[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) least = min(least, v[i]), most = max(most, v[i]);
+  for (int i = 0; i < N; ++i) {
+    v[i] = maxima[threadIdx.x + i * 64];
+    least = min(least, v[i] ? v[i] : ~0u), most = max(most, v[i]);
+  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     least = min(least, (uint32_t)__shfl_xor((int)least, o, 64));
     most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
   }
   uint64_t lo = least, hi = most + 1ull;
-  int n = BLOCK;
+  int n = M;
   while (n > k + spare && hi - lo > 1) {
     const uint32_t mid = (uint32_t)(lo + (hi - lo) / 2);
     int c = 0;
@@ -325,15 +325,19 @@ template <typename T, int BLOCK, int NC>
 __global__ __launch_bounds__(BLOCK)
 __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void top_logits_kernel(
     const T* __restrict__ z, int64_t ld, int V, int k, float c, double inv_t,
-    T* __restrict__ values, int32_t* __restrict__ indices, float* __restrict__ lse) {
+    int cap, T* __restrict__ values, int32_t* __restrict__ indices, float* __restrict__ lse) {
   __shared__ double red[16];
   constexpr int NW = BLOCK / 64, VE = kVE<T>;
   __shared__ struct { float m, base, s; } part[NW];
-  __shared__ uint32_t maxima[BLOCK];
+  constexpr int M = NC > 0 ? BLOCK * NC : BLOCK;   // parts: a chunk each, or a thread's chunks
+  __shared__ uint32_t maxima[M];
   __shared__ uint16_t who[BLOCK];
-  __shared__ uint64_t list[kList];
+  extern __shared__ uint64_t list[];   // [cap]
   __shared__ uint32_t found, who_n, bound;
   const int64_t r = blockIdx.x;
+  // (a wave finds a bound of few maxima sooner, but not one near their number: 8388 x 8000 bf16 by 256
+  // threads' / 1000 chunks' maxima, k 5 44 / 63 us, k 192 235 / 106)
+  const bool chunks = NC > 0 && k > BLOCK / 2;
   Row<T, BLOCK, NC> row;
   row.load(z + r * ld, V);
 
@@ -353,15 +357,23 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void top_logits_kernel(
     for (int j = 0; j < VE; ++j)
       if (f[j] >= low) {
         const uint32_t at = atomicAdd(&found, 1u);
-        if (at < kList) list[at] = order_key(f[j], ch * VE + j);
+        if (at < cap) list[at] = order_key(f[j], ch * VE + j);
         else room = false;
       }
     return room;
   };
   if constexpr (NC > 0) {
-    row.each([&](int, const float* f, auto) {
+    if (chunks) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int ch = threadIdx.x + i * BLOCK;
+        if (ch >= row.n) maxima[ch] = 0;
+      }
+    }
+    row.each([&](int ch, const float* f, auto) {
       first_base<VE>(base, f, c);
-      take(f);
+      const float cm = take(f);
+      if (chunks) maxima[ch] = order_bits(cm);
     });
     if (threadIdx.x == 0) found = who_n = 0;
   } else {
@@ -418,7 +430,7 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void top_logits_kernel(
     __syncthreads();   // (the first part's bound was read; maxima are written again)
   }
   const uint32_t mine = order_bits(m);
-  maxima[threadIdx.x] = mine;
+  if (!chunks) maxima[threadIdx.x] = mine;
   const float wb = wave_fold(base, MaxOp());
   const float ws = wave_fold(s * __builtin_amdgcn_exp2f(base - wb), SumOp());
   m = wave_fold(m, MaxOp());
@@ -445,30 +457,38 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void top_logits_kernel(
     if (threadIdx.x == 0) lse[r] = (float)((double)all * inv_t + log(sum));
   }
 
-  bool few = finite && (int)found >= k && found <= kList;
-  if (!few && finite && k <= BLOCK / 4 * 3) {   // (a thread's maximum passes over NaN)
+  bool few = finite && (int)found >= k && found <= cap;
+  if (!few && finite && k <= (chunks ? row.n / 8 * 5 : BLOCK / 4 * 3)) {   // (a maximum passes over NaN)
     __syncthreads();
     if (threadIdx.x < 64) {
-      const uint32_t v = bound_of_maxima<BLOCK>(maxima, k, k / 4 + 8);
+      const uint32_t v = chunks ? bound_of_maxima<M>(maxima, k, k / 4 + 8)
+                                : bound_of_maxima<BLOCK>(maxima, k, k / 4 + 8);
       if (threadIdx.x == 0) bound = v, found = 0;
     }
     __syncthreads();
     const uint32_t least = bound;
     const float low = float_of(least);
     // (a bound of -inf would take in what pads the row's last chunk)
-    if (mine >= least && low > -INFINITY) who[atomicAdd(&who_n, 1u)] = threadIdx.x;
-    __syncthreads();
-    // the chunks of those threads, read again by all threads at once
-    const int per = (row.n + BLOCK - 1) / BLOCK, items = (int)who_n * per;
-    for (int w = threadIdx.x; w < items; w += BLOCK) {
-      const int ch = who[w / per] + w % per * BLOCK;
-      if (ch >= row.n) continue;
-      float f[VE];
-      unpack(load_chunk(row.p, ch, V), f, T());
-      collect(ch, f, low);
+    if (chunks) {
+      if (low > -INFINITY)
+        row.each([&](int ch, const float* f, auto) {
+          if (chunk_max<VE>(f, -INFINITY) >= low) collect(ch, f, low);
+        });
+    } else {
+      if (mine >= least && low > -INFINITY) who[atomicAdd(&who_n, 1u)] = threadIdx.x;
+      __syncthreads();
+      // the chunks of those threads, read again by all threads at once
+      const int per = (row.n + BLOCK - 1) / BLOCK, items = (int)who_n * per;
+      for (int w = threadIdx.x; w < items; w += BLOCK) {
+        const int ch = who[w / per] + w % per * BLOCK;
+        if (ch >= row.n) continue;
+        float f[VE];
+        unpack(load_chunk(row.p, ch, V), f, T());
+        collect(ch, f, low);
+      }
     }
     __syncthreads();
-    few = (int)found >= k && found <= kList;
+    few = (int)found >= k && found <= cap;
   }
   if (!few) {
     __syncthreads();
@@ -482,7 +502,7 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void top_logits_kernel(
         const uint64_t key = order_key(f[j], idx);
         if (idx < V && key >= b) {
           const uint32_t at = atomicAdd(&found, 1u);
-          if (at < kList) list[at] = key;
+          if (at < cap) list[at] = key;
         }
       }
     });
@@ -911,10 +931,10 @@ void pick_row(int n, int threads, F&& fn) {
   else fn(integral_constant<int, 64>(), integral_constant<int, 1>());
 }
 
-// Rows that do not fill the card (256 CUs of 2048 threads) take more threads each: top_logits of 509
-// rows of 32003 fp32, k 256, by 512 / 1024 threads 45 / 33 us.
-int few_rows(int64_t R, int threads) {
-  while (threads < 1024 && R * threads * 2 <= 256 * 2048) threads *= 2;
+// Rows that do not give each of the 256 CUs `fill` threads take more threads each. top_logits, fill 1024:
+// 509 rows of 32003 fp32, k 16, by 256 / 512 / 1024 threads 21 / 17 / 19 us, k 256 37 / 26 / 26.
+int few_rows(int64_t R, int threads, int fill) {
+  while (threads < 1024 && R * threads * 2 <= 256 * fill) threads *= 2;
   return threads;
 }
 
@@ -949,20 +969,23 @@ void top_logits_launch(const void* logits, int type, int64_t ld, int64_t R, int 
       });
       return;
     }
-    // k maxima of the threads bound the k largest while k is at most three quarters of them. Long rows:
-    // few threads a row leave more rows to hide a row's steps behind, until the first part (four
-    // chunks a thread) is too small a sample. 511 MB, k 64, by 256 / 512 / 1024 threads: 8388 x
-    // 32000 bf16 132 / 149 / 210 us, 2048 x 131072 bf16 132 / 108 / 118, fp32 (1023 MB) 247 / 198 / 185.
-    // Short rows, 67 MB by 64 / 256 threads: 33554 x 2000 bf16, k 100, 584 / 234 us; 67108 x 1000 bf16,
-    // k 100 (125 chunks: too few maxima), 744 / 1827.
+    // Short rows, 134 MB by 64 / 256 threads: 33554 x 2000 bf16, k 5, 52 / 146 us, k 100 128 / 189; 67108
+    // x 1000 bf16, k 192, 271 / 663. Long rows: few threads a row leave more rows to hide a row's steps
+    // behind, until the first part (four chunks a thread) is too small a sample, or its candidates too
+    // many for the threads: by 256 / 512 / 1024 threads 8388 x 32000 bf16, k 64, 124 / 139 / 212, k 512
+    // 404 / 380 / 389; 2048 x 131072 bf16, k 64, 107 / 101 / 113, k 1000 1118 / 450 / 265.
     const int n = (V + kVE<T> - 1) / kVE<T>;
-    const int threads = n <= 1024 ? (k > 48 && k <= 192 && 3 * n >= 4 * k ? 256 : 64)
-                        : few_rows(R, n <= 4096 && k <= 64 ? 256 : n <= 16384 && k <= 384 ? 512 : 1024);
+    const int threads = n <= 1024 ? 64
+                        : few_rows(R, k <= 256 && 8 * k <= n && n <= 8192 ? 256
+                                      : n <= 16384 && (k <= 384 || (k <= 640 && 8 * k <= n)) ? 512 : 1024,
+                                   1024);
     pick_row(n, threads, [&](auto block, auto nc) {
       constexpr int BLOCK = decltype(block)::value, NC = decltype(nc)::value;
+      // (a short row's list is short: its workgroups are small, and LDS would be what limits them)
+      const int cap = NC ? std::min(kList, (3 * k + 255) / 64 * 64) : kList;
       row_parts(R, [&](int64_t r, int64_t rows) {
-        hipLaunchKernelGGL((top_logits_kernel<T, BLOCK, NC>), dim3((uint32_t)rows), dim3(BLOCK), 0, st,
-                           z + r * ld, ld, V, k, c, 1.0 / temp, values + r * k, indices + r * k, lse + r);
+        hipLaunchKernelGGL((top_logits_kernel<T, BLOCK, NC>), dim3((uint32_t)rows), dim3(BLOCK), cap * 8, st,
+                           z + r * ld, ld, V, k, c, 1.0 / temp, cap, values + r * k, indices + r * k, lse + r);
       });
     });
   });
@@ -980,7 +1003,7 @@ void distill_launch(const DistillArgs& a, hipStream_t st) {
     const int n = (a.V + kVE<T> - 1) / kVE<T>;
     const int threads = n <= 1024 ? 64
                                   : few_rows(a.R, a.dz ? (n <= 8192 ? 512 : 1024)
-                                                       : n <= 8192 ? 256 : 512);
+                                                       : n <= 8192 ? 256 : 512, 2048);
     pick_row(n, threads, [&](auto block, auto nc) {
       constexpr int BLOCK = decltype(block)::value, NC = decltype(nc)::value;
       row_parts(a.R, [&](int64_t r, int64_t rows) {

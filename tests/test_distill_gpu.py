@@ -88,6 +88,22 @@ def test_top_logits_hard_rows(v, dtype):
     assert abs(lse[11].item() - 2.0) <= 300 * U
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [130, 500, 2048, 2500, 4000, 8100, 9000, 33000])
+@pytest.mark.parametrize("k", [1, 24, 33, 65, 100, 129, 160, 257, 500, 800, 1024])
+def test_top_logits_on_both_sides_of_each_rule(v, k, dtype):
+    """Bounds by threads' maxima, by chunks', by counting; few threads and many; places counted and
+    searched; rows in random order, ascending, descending, masked at one end, of few values."""
+    z = make(7, v, dtype, 6)
+    z[1] = z[1].sort()[0]
+    z[2] = z[2].sort(descending=True)[0]
+    z[3, v // 3:] = -math.inf
+    z[4, :v // 2] = torch.finfo(dtype).min
+    z[5] = z[5].round()
+    z[6, v // 2] = math.nan
+    check_top(z, min(k, v))
+
+
 def test_top_logits_strided_rows():
     buf = make(9, 1003, torch.bfloat16).cuda()
     for view in (buf[:, 1:778], buf[::2, 3:500], buf[:, :1], buf[2:3].expand(4, 1003), buf.t()):
