@@ -147,7 +147,9 @@ def distill_loss(logits, top, target=None, temperature=1.0, alpha=None, tail=Fal
     loss and gradient 0. ``reduction``: "mean" over all rows, "sum", or "none". A class outside
     the row makes its loss and gradient NaN.
 
-    Teacher's side is data: gradients flow to ``logits`` alone.
+    Teacher's side is data: gradients flow to ``logits`` alone. Forward and backward can be captured,
+    together or apart. As with every autograd function, no eager graph of the same leaves may be alive
+    while a backward is captured.
     """
     if alpha is None:
         if target is not None:

@@ -22,6 +22,9 @@ def gated_linear(x, w_gate, w_up, act="swish"):
     which are rounded to it and whose gradients are fp32. Sums are fp32; in 16 bits the gradients of
     the projections are rounded once to the rows' type, the operand of the products that follow (small
     layers keep them in two parts). In fp16 what overflows there is an infinity.
+
+    Forward and backward can be captured, together or apart. As with every autograd function, no eager
+    graph of the same leaves may be alive while a backward is captured.
     """
     if act not in ACT:
         raise ValueError(f"act must be one of {sorted(a for a in ACT if a)} or None, got {act!r}")
