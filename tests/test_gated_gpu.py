@@ -385,3 +385,22 @@ def test_refusals_on_the_gpu():
             (ValueError, (z(1, (1 << 19) + 8), z(1, (1 << 19) + 8), z(1, (1 << 19) + 8)))]:
         with pytest.raises(err):
             PF.gated_linear(*args)
+
+
+@pytest.mark.parametrize("m, c, f, dtype, wdtype", [
+    (4096, 2048, 5504, torch.bfloat16, None), (1021, 512, 1365, torch.float32, None),
+    (300, 1028, 2056, torch.float16, None), (37, 1000, 2003, torch.bfloat16, torch.float32)])
+def test_same_bits_whatever_the_memory_held(m, c, f, dtype, wdtype):
+    """Every output, workspace and padded copy is written before it is read: the same bits after memory
+    full of NaN, of ones and of zeros."""
+    x, wg, wu, dh = inputs(m, c, f, dtype, 13, wdtype=wdtype)
+    first = None
+    for value in (float("nan"), 1.0, 0.0):
+        torch.cuda.empty_cache()
+        held = [torch.full((n,), value, device="cuda") for n in (1 << 28, 1 << 26, 1 << 24, 1 << 18)]
+        del held                      # (kept by the allocator: what follows is cut out of it)
+        got = run(x, wg, wu, dh, "swish")
+        first = got if first is None else first
+        for a, b in zip(got, first):
+            assert torch.equal(a, b)
+    check(x, wg, wu, dh, "swish", first)
