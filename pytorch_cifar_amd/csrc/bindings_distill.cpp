@@ -71,10 +71,9 @@ struct Loss {
   int64_t ignore_index;
 };
 
-// z [R][V] rows; the rest dense, one entry or K a row -> loss, gradient for a unit seed
-std::tuple<Tensor, Tensor> distill(const Tensor& z, const Tensor& values, const Tensor& indices,
-                                   const Tensor& lse, const Tensor& target, const Loss& l,
-                                   bool want_grad) {
+// z [R][V] rows; the rest dense, one entry or K a row
+DistillArgs args_of(const Tensor& z, const Tensor& values, const Tensor& indices, const Tensor& lse,
+                    const Tensor& target, const Loss& l) {
   DistillArgs a{};
   a.type = logit_type(z);
   a.R = z.size(0);
@@ -93,6 +92,14 @@ std::tuple<Tensor, Tensor> distill(const Tensor& z, const Tensor& values, const 
   a.alpha = l.alpha;
   a.ignore_index = l.ignore_index;
   a.grad_scale = l.reduction == 1 ? (float)(1.0 / std::max<int64_t>(a.R, 1)) : 1.f;
+  return a;
+}
+
+// -> loss, gradient for a unit seed
+std::tuple<Tensor, Tensor> distill(const Tensor& z, const Tensor& values, const Tensor& indices,
+                                   const Tensor& lse, const Tensor& target, const Loss& l,
+                                   bool want_grad) {
+  DistillArgs a = args_of(z, values, indices, lse, target, l);
   const auto f32 = z.options().dtype(at::kFloat);
   auto row_loss = at::empty({a.R}, f32);
   a.row_loss = row_loss.data_ptr<float>();
@@ -119,9 +126,10 @@ int64_t capture() {
 }
 
 // The forward computes the gradient for a unit seed from the row it holds in registers and hands it
-// to the backward, which scales it where the seed is not one. A second backward of a retained graph
-// computes it again from the saved logits, and so does one that is not in the forward's capture: a
-// replay of either alone would scale again what is scaled, or write over what was returned.
+// to the backward, which computes the rows whose seed (read on the device) is not one again from the
+// saved logits: the seed has to come before the rounding. A second backward of a retained graph
+// computes all of them again, and so does one that is not in the forward's capture: a replay of
+// either alone would find rows of another seed, or write over what was returned.
 struct DistillFn : public torch::autograd::Function<DistillFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& values,
                         const Tensor& indices, const optional<Tensor>& lse_,
@@ -150,18 +158,24 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
       auto& d = ctx->saved_data;
       Tensor dz;
       auto it = d.find("dz");
-      if (it != d.end() && capture() == d["capture"].toInt()) {
+      const bool keep = it != d.end() && capture() == d["capture"].toInt();
+      if (keep) {
         dz = it->second.toTensor();
         d.erase(it);
-      } else {
+      }
+      const bool unit = is_unit_seed(grads[0]);
+      if (!keep || !unit) {
         const Loss l{d["temperature"].toDouble(), d["alpha"].toDouble(), d["tail"].toBool(),
                      (int)d["reduction"].toInt(), d["ignore_index"].toInt()};
-        dz = std::get<1>(distill(rows_of(logits), saved[1], saved[2], saved[3], saved[4], l, true));
-      }
-      if (!is_unit_seed(grads[0]) && dz.size(0)) {
+        const Tensor z = rows_of(logits);
+        DistillArgs a = args_of(z, saved[1], saved[2], saved[3], saved[4], l);
         const Tensor s = grads[0].reshape({-1}).contiguous();
-        scale_rows_launch(dz.data_ptr(), logit_type(dz), dz.size(0), (int)dz.size(1),
-                          s.data_ptr<float>(), d["reduction"].toInt() == 0, cur_stream());
+        if (!unit) a.seed = s.data_ptr<float>();
+        a.seed_rows = l.reduction == 0;
+        a.keep = keep;
+        if (!keep) dz = at::empty({a.R, a.V}, z.options());
+        a.dz = dz.data_ptr();
+        if (a.R) distill_launch(a, cur_stream());
       }
       debug_check(d["debug"].toBool(), "distill_loss backward");
       out[0] = dz.view(logits.sizes());

@@ -24,19 +24,19 @@ struct DistillArgs {
   const float* lse;         // [R], read if tail
   const int64_t* target;    // [R] or null
   void* dz;                 // [R][V] dense, or null: no gradient
-  float* row_loss;          // [R]
+  float* row_loss;          // [R], or null: not wanted
+  const float* seed;        // the loss's gradient, [R] or one number for all, or null: ones
   double temp, alpha;       // alpha: weight of the teacher's part
   float grad_scale;         // of every gradient: 1/R for a mean
   int64_t ignore_index;
   int type, value_type;
   int index64, tail;
+  int seed_rows;            // 1: a seed a row
+  int keep;                 // rows of dz whose seed is one are there already
 };
 void distill_launch(const DistillArgs& a, hipStream_t st);
 // loss <- scale * sum of R row losses (fixed order)
 void distill_sum_launch(const float* row_loss, int64_t R, double scale, float* loss,
                         hipStream_t st);
-// dz[r][:] *= s[r * per_row]; rows whose factor is 1 are left alone
-void scale_rows_launch(void* dz, int type, int64_t R, int V, const float* s, int per_row,
-                       hipStream_t st);
 
 }  // namespace pca

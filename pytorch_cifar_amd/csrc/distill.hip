@@ -599,6 +599,9 @@ __global__ __launch_bounds__(256) void top_small_kernel(const T* __restrict__ z,
 // cache behind the L2s. 4096 x 128000 bf16, k 64, with rest and labels, 475 us (4.4 TB/s of 2.1 GB);
 // the loss alone of 2000 x 50257 fp16 50 us (4.0 TB/s).
 //
+// The loss's own gradient multiplies a row's in fp32 and 64 bits, before its one rounding: under a loss
+// scale (fp16) most shares of a long row have no 16-bit number without it.
+//
 // The label's softmax is at temperature 1. Where T is 2 or 4 its exponentials are powers of those at
 // T, which saves the second quarter-rate instruction of a class and pass.
 struct Sums {
@@ -619,6 +622,8 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void distill_kernel(Distil
   __shared__ int flags[4];     // kept entries with mass, an index twice, an index past the classes
   const int64_t r = blockIdx.x;
   const int V = a.V, K = a.K, t = threadIdx.x, wave = t >> 6;
+  const float seed = GRAD && a.seed ? a.seed[r * a.seed_rows] : 1.f;
+  if (GRAD && a.keep && seed == 1.f) return;
   double* p = reinterpret_cast<double*>(smem);          // [K] the teacher's probabilities
   float* zk = reinterpret_cast<float*>(p + K);          // [K] the student's logits there
   int* cls = reinterpret_cast<int*>(zk + K);            // [K] their classes, -1: not kept
@@ -668,7 +673,7 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void distill_kernel(Distil
   T* dr = GRAD ? reinterpret_cast<T*>(a.dz) + r * V : nullptr;
   if (poison || (!kd && !label)) {   // without a term the row's logits do not count
     const float v = poison ? __builtin_nanf("") : 0.f;
-    if (t == 0) a.row_loss[r] = v;
+    if (t == 0 && a.row_loss) a.row_loss[r] = v;
     if constexpr (GRAD) {
       float f[VE];
 #pragma unroll
@@ -815,7 +820,7 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void distill_kernel(Distil
       kl = wave_fold(kl, SumOp()) * kLn2 + side[2] + mass * log(all);
       if (rest > 0) kl += rest * (log(rest) - log(left / all));
     }
-    if (t == 0) {
+    if (t == 0 && a.row_loss) {
       double loss = kd ? kl * at2 * a.temp : 0;
       if (label) {
         const float c1 = two ? kLog2e : ct;
@@ -828,7 +833,7 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void distill_kernel(Distil
   }
   if constexpr (!GRAD) return;
 
-  const double gs = a.grad_scale;
+  const double gs = (double)a.grad_scale * seed;
   const double A = kd ? gs * at2 * (mass + rest) / all : 0.0;
   const double B = rest > 0 && left > 0 ? gs * at2 * rest / left : 0.0;
   const double D = label ? gs * (1 - a.alpha) / total1 : 0.0;
@@ -900,24 +905,6 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restri
   for (int64_t i = threadIdx.x; i < n; i += 1024) s += v[i];
   s = block_fold<1024>(s, red, SumOp());
   if (threadIdx.x == 0) out[0] = (float)(s * scale);
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void scale_rows_kernel(T* __restrict__ dz, int64_t R, int V,
-                                                         const float* __restrict__ s, int per_row) {
-  for (int64_t r = blockIdx.x; r < R; r += gridDim.x) {
-    const float g = s[r * per_row];
-    if (g == 1.f) continue;
-    T* p = dz + r * V;
-    for (int c = threadIdx.x; c * kVE<T> < V; c += 256) {
-      const uint4 u = load_chunk(p, c, V);
-      float f[kVE<T>];
-      unpack(u, f, T());
-#pragma unroll
-      for (int j = 0; j < kVE<T>; ++j) f[j] *= g;
-      store_chunk(p, c, V, f);
-    }
-  }
 }
 
 // Threads and register chunks of a row of n chunks: calls fn<BLOCK, NC>. Up to 1024 chunks are held in
@@ -1017,7 +1004,8 @@ void distill_launch(const DistillArgs& a, hipStream_t st) {
         if (a.lse) b.lse = a.lse + r;
         if (a.target) b.target = a.target + r;
         if (a.dz) b.dz = reinterpret_cast<T*>(a.dz) + r * a.V;
-        b.row_loss = a.row_loss + r;
+        if (a.row_loss) b.row_loss = a.row_loss + r;
+        if (a.seed) b.seed = a.seed + r * a.seed_rows;
         if (a.dz)
           hipLaunchKernelGGL((distill_kernel<T, BLOCK, NC, true>), dim3((uint32_t)rows), dim3(BLOCK),
                              lds, st, b, c_t);
@@ -1032,16 +1020,6 @@ void distill_launch(const DistillArgs& a, hipStream_t st) {
 void distill_sum_launch(const float* row_loss, int64_t R, double scale, float* loss,
                         hipStream_t st) {
   hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, st, row_loss, R, scale, loss);
-}
-
-void scale_rows_launch(void* dz, int type, int64_t R, int V, const float* s, int per_row,
-                       hipStream_t st) {
-  const uint32_t grid = (uint32_t)std::min<int64_t>(R, 4096);
-  pick_type(type, [&](auto tv) {
-    using T = decltype(tv);
-    hipLaunchKernelGGL((scale_rows_kernel<T>), dim3(grid), dim3(256), 0, st,
-                       reinterpret_cast<T*>(dz), R, V, s, per_row);
-  });
 }
 
 }  // namespace pca

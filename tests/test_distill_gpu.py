@@ -523,3 +523,56 @@ def test_refuses_what_does_not_fit():
             (ValueError, (torch.zeros(1, (1 << 18) + 1, device="cuda"), 1), {})]:
         with pytest.raises(err):
             PF.top_logits(*args, **kw)
+
+
+def oracle_on_gpu(z, top, y, t, alpha, tail, seeds):
+    """oracle() on the GPU, for rows too many for the CPU."""
+    x = z.detach().double().requires_grad_(True)
+    loss = _ref_distill(x, *top, y, t, alpha, tail, -100)
+    (g,) = torch.autograd.grad((loss * seeds.double()).sum(), x)
+    return loss.detach(), g
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("r, v, tail", [(2048, 4099, False), (1500, 9001, True)])
+def test_seeds_reach_the_gradient_before_its_rounding(r, v, tail, dtype):
+    """A loss scale of 2^16 over the mean, and a seed a row: one rounding, of what the seed has
+    multiplied. (The shares of thousands of classes, divided by the rows, are below fp16's numbers.)"""
+    t, k, alpha = 2.0, 16, 0.5
+    z, top, y = distill_inputs(r, v, k, dtype, t)
+    z, top, y = z.cuda(), gpu_top(top), y.cuda()
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x = z.detach().requires_grad_(True)
+    kw = dict(temperature=t, alpha=alpha, tail=tail)
+    each = torch.exp2(torch.randint(-8, 17, (r,), generator=g, device="cuda").float()) / r
+    each[::5] = 1.0
+    for reduction, seed, rows in (("mean", torch.tensor(65536.0, device="cuda"), torch.full((r,), 65536.0 / r)),
+                                  ("none", each, each)):
+        loss = PF.distill_loss(x, top, y, reduction=reduction, **kw)
+        (got,) = torch.autograd.grad(loss, x, seed)
+        rows = rows.cuda()
+        _, want = oracle_on_gpu(z, top, y, t, alpha, tail, rows)
+        c = (3 * spread(z, t) + 260) * U
+        q = alpha * t * torch.softmax(z.double() / t, 1) + (1 - alpha) * torch.softmax(z.double(), 1)
+        tol = (2 * c * (q * rows.double()[:, None] + want.abs()) + torch.finfo(dtype).eps / 2 * want.abs()
+               + (2.0 ** -25 if dtype == torch.float16 else 1e-37))
+        assert ((got.double() - want).abs() <= tol).all()
+        if dtype == torch.float16 and reduction == "mean":
+            # what half of the smallest number is reached by is not zero
+            assert (got[want.abs() > 2.0 ** -24] != 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_seed_of_one_is_the_unit_seed(dtype):
+    z, top, y = distill_inputs(70, 1003, 9, dtype, 2.0)
+    top, y = gpu_top(top), y.cuda()
+    kw = dict(temperature=2.0, alpha=0.5, tail=True)
+    x = z.cuda().requires_grad_(True)
+    grads = []
+    for seed in ("unit", None, 1.0, "again"):
+        loss = PF.distill_loss(x, top, y, **kw)
+        s = PF.unit_grad(loss) if seed in ("unit", "again") else None if seed is None else torch.tensor(1.0, device="cuda")
+        if seed == "again":
+            torch.autograd.grad(loss, x, s, retain_graph=True)
+        grads.append(torch.autograd.grad(loss, x, s)[0])
+    assert all(torch.equal(g, grads[0]) for g in grads)
