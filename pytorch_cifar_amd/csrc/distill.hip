@@ -592,6 +592,10 @@ __global__ __launch_bounds__(256) void top_small_kernel(const T* __restrict__ z,
 // kept classes hold nearly all). The K values of the teacher's side are computed in 64 bits: what
 // is left of its mass, 1 - sum p, is a difference.
 //
+// Where the kept classes stand so far above all others (41 in z/T) that s_rest is less than 2^-60 of the
+// base, the rest is summed again against its own maximum, which costs two more passes: terms below 2^-126
+// of a base are zero in 32 bits, and so shares e_j / s_rest below 2^-66 are all that is lost.
+//
 // A bit a class marks the kept ones (LDS, V / 8 bytes). It gives s_rest, and finds an index that
 // a row names twice: its entries are then gathered for each of them.
 //
@@ -604,6 +608,7 @@ __global__ __launch_bounds__(256) void top_small_kernel(const T* __restrict__ z,
 //
 // The label's softmax is at temperature 1. Where T is 2 or 4 its exponentials are powers of those at
 // T, which saves the second quarter-rate instruction of a class and pass.
+constexpr double kFaint = 1 / kMost;   // 2^-60
 struct Sums {
   float base, base1;         // at T, at temperature 1
   float rest, kept, one;     // of e over the classes not kept, the kept ones; of all at 1
@@ -805,6 +810,31 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void distill_kernel(Distil
   const double all = left + inner;
   if (!two) total1 = all;
   const double mass = kd ? side[0] : 0, rest = kd ? side[1] : 0;
+  // log of the rest's share; far: its exponentials are against mr, the largest of its classes
+  double lrest = 0;
+  float mr = -INFINITY;
+  bool far = rest > 0 && left < kFaint;
+  if (far) {
+    auto others = [&](auto&& fn) {
+      row.each([&](int c, const float* f, auto) {
+        const uint32_t bits = mark8[c * VE >> 3] >> (c * VE & 7);
+#pragma unroll
+        for (int j = 0; j < VE; ++j)
+          if (!(bits >> j & 1)) fn(f[j]);
+      });
+    };
+    others([&](float z) { mr = fmaxf(mr, z); });
+    mr = block_fold<BLOCK>(mr, reinterpret_cast<float*>(red), MaxOp());
+    far = mr != -INFINITY;   // (no mass at all: log 0)
+    if (far) {
+      float sr = 0.f;
+      others([&](float z) { sr += term_at(z, mr, ct); });
+      left = block_fold<BLOCK>((double)sr, red, SumOp());
+      const double x = plain ? ((double)mr - (double)m) * (double)ct : (double)mr * (double)ct - (double)b;
+      lrest = x * kLn2 + log(left) - log(all);
+    }
+  }
+  if (rest > 0 && !far) lrest = log(left / all);
   const double at2 = a.alpha * a.temp;
 
   if (wave == 0) {
@@ -818,7 +848,7 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void distill_kernel(Distil
         kl -= p[k] * x;
       }
       kl = wave_fold(kl, SumOp()) * kLn2 + side[2] + mass * log(all);
-      if (rest > 0) kl += rest * (log(rest) - log(left / all));
+      if (rest > 0) kl += rest * (log(rest) - lrest);
     }
     if (t == 0 && a.row_loss) {
       double loss = kd ? kl * at2 * a.temp : 0;
@@ -835,10 +865,21 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void distill_kernel(Distil
 
   const double gs = (double)a.grad_scale * seed;
   const double A = kd ? gs * at2 * (mass + rest) / all : 0.0;
-  const double B = rest > 0 && left > 0 ? gs * at2 * rest / left : 0.0;
+  const double Br = rest > 0 && left > 0 ? gs * at2 * rest / left : 0.0;
+  const double B = far ? 0.0 : Br;   // (far: a term of its own, at its own base)
   const double D = label ? gs * (1 - a.alpha) / total1 : 0.0;
   const float ca = (float)(two ? A - B : A - B + D), cd = (float)D;
-  if (plain) {
+  if (far) {
+    row.each([&](int c, const float* f, auto whole) {
+      float g[VE];
+#pragma unroll
+      for (int j = 0; j < VE; ++j) {
+        g[j] = ca * (plain ? term_at(f[j], m, ct) : term(f[j], ct, b)) - (float)Br * term_at(f[j], mr, ct);
+        if (two) g[j] += cd * (plain ? term_at(f[j], m, kLog2e) : term(f[j], kLog2e, b1));
+      }
+      store_chunk<NC == 0>(dr, c, V, g, whole);
+    });
+  } else if (plain) {
     row.each([&](int c, const float* f, auto whole) {
       float g[VE];
 #pragma unroll
@@ -873,8 +914,9 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void distill_kernel(Distil
   // the kept classes and the label's, after the plain values above are written
   __syncthreads();
   const bool dup = flags[1] != 0;
-  auto fix = [&](int j, float z, double share, double pk) {
+  auto fix = [&](int j, float z, double share, double pk, bool kept) {
     double g = -gs * at2 * pk;
+    if (far && !kept) g -= Br * term_at(z, mr, ct);
     if (kd) g += share * (plain ? term_at(z, m, ct) : term(z, ct, b));
     if (label) {
       const float c1 = two ? kLog2e : ct;
@@ -892,10 +934,10 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void distill_kernel(Distil
         for (int i = 0; i < K; ++i)
           if (cls[i] == cls[k]) pk += p[i];
       }
-      fix(cls[k], zk[k], A, pk);
+      fix(cls[k], zk[k], A, pk, true);
     }
   }
-  if (label && t == 0 && !(kd && (mark[y >> 5] >> (y & 31) & 1))) fix((int)y, zy, A - B, 0.0);
+  if (label && t == 0 && !(kd && (mark[y >> 5] >> (y & 31) & 1))) fix((int)y, zy, A - B, 0.0, false);
 }
 
 __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restrict__ v, int64_t n,

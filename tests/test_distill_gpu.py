@@ -576,3 +576,66 @@ def test_a_seed_of_one_is_the_unit_seed(dtype):
             torch.autograd.grad(loss, x, s, retain_graph=True)
         grads.append(torch.autograd.grad(loss, x, s)[0])
     assert all(torch.equal(g, grads[0]) for g in grads)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [70, 1000, 9000, 70000])
+@pytest.mark.parametrize("t, labels, k", [(1.0, False, 1), (2.0, True, 3), (0.7, True, 1), (0.1, False, 3)])
+def test_rest_far_below_the_kept(v, dtype, t, labels, k):
+    """A student whose kept classes stand far above all others (gaps in z / T): the rest's mass has a
+    logarithm and shares where it is too small a part of the row for 32 bits."""
+    gaps = [30.0, 50.0, 54.0, 57.0, 62.0, 80.0, 86.0, 90.0, 100.0, 200.0, 700.0, 100.0]
+    r, alpha = len(gaps), 0.6 if labels else 1.0
+    z = make(r, v, torch.float32, 21, 1.0)
+    idx = torch.stack([torch.randperm(v, generator=torch.Generator().manual_seed(i))[:k] for i in range(r)])
+    z.scatter_(1, idx, (torch.tensor(gaps)[:, None] + torch.arange(k)) * t)
+    z[11] = -math.inf                       # nothing but the kept and one more
+    z[11, idx[11]] = 3.0
+    z[11, (idx[11, 0] + 1) % v if k == 1 else next(j for j in range(v) if j not in idx[11].tolist())] = 3.0 - 150 * t
+    z = z.to(dtype)
+    values = t * torch.arange(k).float().expand(r, k).contiguous()
+    # the kept classes hold 0.99 of the teacher's mass
+    lse = torch.logsumexp(values.double() / t, 1).sub(math.log(0.99)).float()
+    top = PF.TopLogits(values, idx.int(), lse)
+    y = None
+    if labels:
+        y = idx[:, 0].clone()
+        y[1::2] = (y[1::2] + 1) % v         # (some are kept classes, most of these are not)
+        y[11] = idx[11, 0]
+    want, grad = oracle(z, top, y, t, alpha, True)
+    x = z.cuda().requires_grad_(True)
+    kw = dict(temperature=t, alpha=alpha, tail=True, reduction="none")
+    loss = PF.distill_loss(x, gpu_top(top), y.cuda() if labels else None, **kw)
+    loss.backward(torch.ones_like(loss))
+    alone = PF.distill_loss(x.detach(), gpu_top(top), y.cuda() if labels else None, **kw)
+    for i in range(r):
+        tl, tg = tolerances(z[i:i + 1], t, alpha, grad[i:i + 1])
+        for got in (loss, alone):
+            assert abs(got[i].item() - want[i].item()) <= tl + 2 * U * want[i].abs(), (i, got[i], want[i])
+        off = (x.grad[i].cpu().double() - grad[i]).abs()
+        # Exponentials below 2^-126 of their base are zero in 32 bits. The rest's mass is 2^-60 of its base
+        # at least (it takes another below), so what is zero has a share of the rest below 2^-66, and
+        # alpha T rest times it of the gradient; the teacher's rest is 0.01.
+        lost = alpha * t * 0.01 * 2.0 ** -66
+        assert (off <= tg(dtype)[0] + lost).all(), (i, off.max())
+
+
+def test_rest_without_classes():
+    """All other classes masked by -inf: the teacher gives them mass, the student none."""
+    z = torch.full((2, 300), -math.inf)
+    z[:, 5] = 1.0
+    z[1, 6:] = torch.finfo(torch.float32).min
+    top = PF.TopLogits(torch.zeros(2, 1), torch.full((2, 1), 5, dtype=torch.int32), torch.full((2,), 0.01))
+    want, _ = oracle(z, top, None, 1.0, 1.0, True)
+    x = z.cuda().requires_grad_(True)
+    loss = PF.distill_loss(x, gpu_top(top), tail=True, reduction="none")
+    loss.backward(torch.ones_like(loss))
+    assert loss[0] == math.inf
+    # (the rest's logarithm is the mask's value over T: all but the rest's share of it is rounding)
+    assert abs(loss[1].item() / want[1].item() - 1) <= 8 * U
+    # the student's mass is all at class 5 (q = 1, p = 1 - rest), that of the others is shared by the 294
+    # that are not at -inf alike: gradients rest and -rest / 294
+    rest = 1 - math.exp(-top.lse[1].item())
+    by_hand = torch.zeros(300, dtype=torch.float64)
+    by_hand[5], by_hand[6:] = rest, -rest / 294
+    assert ((x.grad[1].cpu().double() - by_hand).abs() <= 600 * U * by_hand.abs()).all()
