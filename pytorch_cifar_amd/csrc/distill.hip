@@ -196,9 +196,11 @@ __device__ __forceinline__ A block_fold(A v, A* red, Op op) {
 
 // Sum of 2^(x - base) over a thread's x = z c, in one pass without the maximum: a term costs one
 // multiply-add, the exponential and the add. The base is the first chunk's largest x, as a whole
-// number (sums of different bases are joined by exact powers of two): 2^60 above and all below it
-// is room for what follows. A row that leaves it (a first chunk of masked classes, |x| past 2^22,
-// infinities, NaN) is summed again against its maximum (`plain` below).
+// number: sums of different bases are joined by exact powers of two, which meet the sum before it is
+// rounded (a thread's may be 2^127 above its base, and the base more than that below the row's: 2^-130 as
+// a factor would be zero). 2^60 above and all below it is room for what follows. A row that leaves it (a
+// first chunk of masked classes, |x| past 2^22, infinities, NaN) is summed again against its maximum
+// (`plain` below).
 constexpr float kNoBase = -4194304.f, kFar = 4194304.f;
 constexpr double kMost = 1152921504606846976.0;   // 2^60
 
@@ -434,7 +436,7 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void top_logits_kernel(
   const uint32_t mine = order_bits(m);
   if (!chunks) maxima[threadIdx.x] = mine;
   const float wb = wave_fold(base, MaxOp());
-  const float ws = wave_fold(s * __builtin_amdgcn_exp2f(base - wb), SumOp());
+  const float ws = wave_fold(ldexpf(s, (int)(base - wb)), SumOp());
   m = wave_fold(m, MaxOp());
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = {m, wb, ws};
   __syncthreads();
@@ -442,7 +444,7 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void top_logits_kernel(
   const auto mp = part[threadIdx.x & (NW - 1)];
   float all = wave_fold<NW>(mp.m, MaxOp());
   const float b = wave_fold<NW>(mp.base, MaxOp());
-  double sum = wave_fold<NW>((double)mp.s * __builtin_amdgcn_exp2f(mp.base - b), SumOp());
+  double sum = wave_fold<NW>(ldexp((double)mp.s, (int)(mp.base - b)), SumOp());
   bool finite = true;   // no NaN in the row
   if (sum > 0 && sum < kMost) {
     if (threadIdx.x == 0) lse[r] = (float)(((double)b + log2(sum)) * 0.6931471805599453);
@@ -766,24 +768,24 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void distill_kernel(Distil
   if (power) base1 = s.base * power;
   // sums of the threads, in a fixed order: each wave's at its own base, then all of them
   const float wb = wave_fold(s.base, MaxOp()), wb1 = wave_fold(base1, MaxOp());
-  auto join = [&](float scale, float scale1) {
-    const Sums w = {wb, wb1, wave_fold(s.rest * scale, SumOp()), wave_fold(s.kept * scale, SumOp()),
-                    wave_fold(s.one * scale1, SumOp())};
+  auto join = [&](int d, int d1) {
+    const Sums w = {wb, wb1, wave_fold(ldexpf(s.rest, d), SumOp()), wave_fold(ldexpf(s.kept, d), SumOp()),
+                    wave_fold(ldexpf(s.one, d1), SumOp())};
     __syncthreads();
     if ((t & 63) == 0) part[wave] = w;
     __syncthreads();
   };
-  join(__builtin_amdgcn_exp2f(s.base - wb), two ? __builtin_amdgcn_exp2f(base1 - wb1) : 0.f);
+  join((int)(s.base - wb), (int)(base1 - wb1));
   // (a wave's part a lane: every wave joins them for itself)
   Sums v = part[t & (NW - 1)];
   const float b = wave_fold<NW>(v.base, MaxOp()), b1 = wave_fold<NW>(v.base1, MaxOp());
   double left = 0, inner = 0, total1 = 0;
-  auto total = [&](float scale, float scale1) {
-    left = wave_fold<NW>((double)v.rest * scale, SumOp());
-    if (tail) inner = wave_fold<NW>((double)v.kept * scale, SumOp());
-    if (two) total1 = wave_fold<NW>((double)v.one * scale1, SumOp());
+  auto total = [&](int d, int d1) {
+    left = wave_fold<NW>(ldexp((double)v.rest, d), SumOp());
+    if (tail) inner = wave_fold<NW>(ldexp((double)v.kept, d), SumOp());
+    if (two) total1 = wave_fold<NW>(ldexp((double)v.one, d1), SumOp());
   };
-  total(__builtin_amdgcn_exp2f(v.base - b), __builtin_amdgcn_exp2f(v.base1 - b1));
+  total((int)(v.base - b), (int)(v.base1 - b1));
   // plain: exponentials against the row's maximum, for both temperatures
   const double sum = left + inner;
   const bool plain = !(sum > 0 && sum < kMost && (!two || (total1 > 0 && total1 < kMost)));
@@ -803,9 +805,9 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void distill_kernel(Distil
         for (int j = 0; j < VE; ++j) s.one += term_at(f[j], m, kLog2e);
       }
     });
-    join(1.f, 1.f);
+    join(0, 0);
     v = part[t & (NW - 1)];
-    total(1.f, 1.f);
+    total(0, 0);
   }
   const double all = left + inner;
   if (!two) total1 = all;

@@ -639,3 +639,27 @@ def test_rest_without_classes():
     by_hand = torch.zeros(300, dtype=torch.float64)
     by_hand[5], by_hand[6:] = rest, -rest / 294
     assert ((x.grad[1].cpu().double() - by_hand).abs() <= 600 * U * by_hand.abs()).all()
+
+
+@pytest.mark.parametrize("v", [300, 1000, 2000, 8192, 40000, 150000])
+@pytest.mark.parametrize("low", [-86.0, -88.0, -89.0, -90.0, -95.0, -100.0])
+def test_first_chunks_far_below_the_rest(v, low):
+    """The classes that threads meet first stand some 90 below the largest, what follows them near it: a
+    thread's sum is far above its base, and its base as far below the row's."""
+    for first in (64 * 4, 256 * 4, 1024 * 4):
+        z = make(6, v, torch.float32, 31, 0.5) - 10.0
+        z[:, :first] = low
+        z[2:4] = torch.where(torch.arange(v) < first, low, -14.0)
+        z[:, 5] = 0.0
+        z[1, 5], z[1, v - 1] = low, 0.0
+        check_top(z, min(v, 7))
+        top = PF.TopLogits(torch.zeros(6, 1), torch.full((6, 1), v // 2, dtype=torch.int32), torch.full((6,), 0.5))
+        y = torch.full((6,), v - 1)
+        for t, tail in ((1.0, True), (2.0, False), (0.9, True)):
+            want, grad = oracle(z, top, y, t, 0.5, tail)
+            tl, tg = tolerances(z, t, 0.5, grad)
+            x = z.cuda().requires_grad_(True)
+            loss = PF.distill_loss(x, gpu_top(top), y.cuda(), temperature=t, alpha=0.5, tail=tail, reduction="none")
+            loss.backward(torch.ones_like(loss))
+            assert ((loss.cpu().double() - want).abs() <= tl + 2 * U * want.abs()).all()
+            assert ((x.grad.cpu().double() - grad).abs() <= tg(torch.float32)).all()
