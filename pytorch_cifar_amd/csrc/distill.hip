@@ -204,11 +204,16 @@ __device__ __forceinline__ A block_fold(A v, A* red, Op op) {
 constexpr float kNoBase = -4194304.f, kFar = 4194304.f;
 constexpr double kMost = 1152921504606846976.0;   // 2^60
 
-template <int N>
-__device__ __forceinline__ void first_base(float& base, const float* f, float c) {
+// (What was summed before a base was found is relative to kNoBase: masks of some -2^22, or nothing.
+// scale(d): shift those sums by 2^d)
+template <int N, typename F>
+__device__ __forceinline__ void first_base(float& base, const float* f, float c, F&& scale) {
   if (base != kNoBase) return;
   const float x = chunk_max<N>(f, f[0]) * c;
-  if (x > kNoBase && x < kFar) base = rintf(x);
+  if (x > kNoBase && x < kFar) {
+    base = rintf(x);
+    scale((int)(kNoBase - base));
+  }
 }
 
 __device__ __forceinline__ float term(float z, float c, float base) {
@@ -346,6 +351,7 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void top_logits_kernel(
   row.load(z + r * ld, V);
 
   float m = -INFINITY, base = kNoBase, s = 0.f;
+  auto found_base = [&](int d) { s = ldexpf(s, d); };
   auto take = [&](const float* f) {
     const float cm = chunk_max<VE>(f, -INFINITY);
     m = fmaxf(m, cm);
@@ -375,7 +381,7 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void top_logits_kernel(
       }
     }
     row.each([&](int ch, const float* f, auto) {
-      first_base<VE>(base, f, c);
+      first_base<VE>(base, f, c, found_base);
       const float cm = take(f);
       if (chunks) maxima[ch] = order_bits(cm);
     });
@@ -397,7 +403,7 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void top_logits_kernel(
     for (int j = 0; j < A; ++j)
       if (t + j * BLOCK < row.n) {
         unpack(v[j], f, T());
-        first_base<VE>(base, f, c);
+        first_base<VE>(base, f, c, found_base);
         take(f);
       }
     maxima[t] = order_bits(m);
@@ -754,13 +760,17 @@ __attribute__((amdgpu_waves_per_eu(NC == 0 ? 8 : 1))) void distill_kernel(Distil
     }
   };
   row.each([&](int c, const float* f, auto) {
-    first_base<VE>(s.base, f, ct);
+    first_base<VE>(s.base, f, ct, [&](int d) {
+      s.rest = ldexpf(s.rest, d);
+      s.kept = ldexpf(s.kept, d);
+      if (power) s.one = ldexpf(s.one, power * d);
+    });
     float e[VE];
 #pragma unroll
     for (int j = 0; j < VE; ++j) e[j] = term(f[j], ct, s.base);
     add(c, e);
     if (two && !power) {
-      first_base<VE>(base1, f, kLog2e);
+      first_base<VE>(base1, f, kLog2e, [&](int d) { s.one = ldexpf(s.one, d); });
 #pragma unroll
       for (int j = 0; j < VE; ++j) s.one += term(f[j], kLog2e, base1);
     }

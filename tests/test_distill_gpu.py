@@ -663,3 +663,29 @@ def test_first_chunks_far_below_the_rest(v, low):
             loss.backward(torch.ones_like(loss))
             assert ((loss.cpu().double() - want).abs() <= tl + 2 * U * want.abs()).all()
             assert ((x.grad.cpu().double() - grad).abs() <= tg(torch.float32)).all()
+
+
+@pytest.mark.parametrize("v", [300, 2000, 9000, 40000])
+@pytest.mark.parametrize("t", [1.0, 2.0, 0.5])
+def test_classes_masked_by_some_millions(v, t):
+    """Masks near -2^22 / log2(e) T, below which a thread takes no base from its first classes: what it
+    has summed by then counts as little as before."""
+    z = make(12, v, torch.float32, 41, 1.0)
+    for i, steps in enumerate((-200.0, -100.0, -20.0, -4.0, -1.0, -0.5, 0.0, 0.5, 1.0, 20.0, 200.0, -126.0)):
+        z[i, :v - 40] = (steps - 4194304.0) / 1.4426950408889634 * t
+    real = z[:, v - 40:]
+    lse = PF.top_logits(z.cuda(), 7, t).lse.cpu().double()
+    ref = torch.logsumexp(z.double() / t, 1)
+    # (the row's own classes spread over some 10: what is masked has a share of 0, with any error)
+    assert ((lse - ref).abs() <= (3 * spread(real, t) + 260) * U + U * ref.abs()).all()
+    top = PF.TopLogits(torch.zeros(12, 1), torch.full((12, 1), v - 3, dtype=torch.int32), torch.full((12,), 0.5))
+    y = torch.full((12,), v - 1)
+    for tail in (False, True):
+        want, grad = oracle(z, top, y, t, 0.5, tail)
+        tl, tg = tolerances(real, t, 0.5, grad[:, v - 40:])
+        x = z.cuda().requires_grad_(True)
+        loss = PF.distill_loss(x, gpu_top(top), y.cuda(), temperature=t, alpha=0.5, tail=tail, reduction="none")
+        loss.backward(torch.ones_like(loss))
+        assert ((loss.cpu().double() - want).abs() <= tl + 2 * U * want.abs()).all()
+        assert ((x.grad.cpu().double() - grad).abs()[:, v - 40:] <= tg(torch.float32)).all()
+        assert not x.grad[:, :v - 40].any()
