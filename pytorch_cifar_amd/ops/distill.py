@@ -115,7 +115,11 @@ def _ref_distill(z, values, indices, lse, target, t, alpha, tail, ignore_index):
         some = rest != 0
         outer = logq.masked_fill(inside, -math.inf)
         outer = torch.where(some[:, None], outer, torch.zeros_like(outer))
-        lrest = torch.logsumexp(outer, 1)
+        # (the logarithm of the sum apart from its base: where all other classes are masked by the type's
+        # lowest value it is below the base's last bit, and their shares with it)
+        shift = outer.detach().amax(1, keepdim=True)
+        shift = torch.where(torch.isfinite(shift), shift, torch.zeros_like(shift))
+        lrest = (outer - shift).exp().sum(1).log() + shift[:, 0]
         loss = loss + torch.where(some, rest * (torch.where(some, rest, torch.ones_like(rest)).log()
                                                 - lrest), torch.zeros_like(rest))
     loss = torch.where(has, loss * (alpha * t * t), torch.zeros_like(loss))

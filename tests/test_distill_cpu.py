@@ -197,3 +197,17 @@ def test_distill_refuses_what_does_not_fit():
 def test_top_logits_refusals(z, k, kw, err):
     with pytest.raises(err):
         PF.top_logits(z, k, **kw)
+
+
+def test_gradient_of_the_rest_under_a_mask():
+    """All classes but the kept one masked by the type's lowest value: the mass that the teacher leaves to
+    them is shared by them alike."""
+    z = torch.full((1, 300), torch.finfo(torch.float32).min)
+    z[0, 5] = 1.0
+    top = PF.TopLogits(torch.zeros(1, 1), torch.full((1, 1), 5, dtype=torch.int32), torch.full((1,), 0.01))
+    z.requires_grad_(True)
+    PF.distill_loss(z, top, tail=True).backward()
+    rest = 1 - math.exp(-top.lse.item())
+    want = torch.full((300,), -rest / 299, dtype=torch.float64)
+    want[5] = rest                          # (q = 1 there, and p = 1 - rest)
+    assert ((z.grad[0].double() - want).abs() <= 2 * HALF * want.abs()).all()
