@@ -653,6 +653,11 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GatedArgs a, int64_t n)
 
 // ------------------------------------------------------------------------ elementwise passes
 // dg and du. Bound by the bytes: 4096 x 5504 bf16 (316 MB) 66 us, the rate of a large copy.
+//
+// Two parts, a number and what it was rounded by, are as good as their sum in products with finite
+// numbers; with an infinity the second gives one of the other sign, or NaN. An infinity in a row or a
+// weight makes every projection that its product with dg or du belongs to infinite or NaN, so there, and
+// where dg or du is one itself, both parts are half of the rounded number.
 template <typename E>
 __global__ __launch_bounds__(256) void gated_dact_kernel(const float* __restrict__ g,
                                                          const float* __restrict__ u,
@@ -665,6 +670,7 @@ __global__ __launch_bounds__(256) void gated_dact_kernel(const float* __restrict
     const int64_t m = w / pieces;
     const int f0 = (int)(w % pieces) * PC;
     E dg[PC], du[PC];
+    bool wild[PC];
     float gv[PC], uv[PC];
     E d[PC];
     if (f0 + PC <= F) {
@@ -685,24 +691,32 @@ __global__ __launch_bounds__(256) void gated_dact_kernel(const float* __restrict
       const float df = static_cast<float>(d[i]);
       float v, slope;
       act_both(gv[i], act, v, slope);
+      wild[i] = !isfinite(gv[i]) || !isfinite(uv[i]);
       gv[i] = df * uv[i] * slope;
       uv[i] = df * v;
       dg[i] = static_cast<E>(gv[i]);
       du[i] = static_cast<E>(uv[i]);
     }
     E* row = out + m * 2 * parts * Fp + f0;
-    __builtin_memcpy(row, dg, 16);
-    __builtin_memcpy(row + Fp, du, 16);
-    if (parts == 2) {   // (of an infinity nothing is left)
+    if (parts == 2) {
+      E dg2[PC], du2[PC];
+      auto rest = [&](E& first, float v, bool far) {
+        const float r = static_cast<float>(first);
+        if (!far && !isinf(r)) return static_cast<E>(v - r);
+        const E half = static_cast<E>(r * 0.5f);
+        if (static_cast<float>(half) != 0.f) first = half;   // (the smallest number is counted twice)
+        return first;
+      };
 #pragma unroll
       for (int i = 0; i < PC; ++i) {
-        const float g0 = static_cast<float>(dg[i]), u0 = static_cast<float>(du[i]);
-        dg[i] = static_cast<E>(isinf(g0) ? 0.f : gv[i] - g0);
-        du[i] = static_cast<E>(isinf(u0) ? 0.f : uv[i] - u0);
+        dg2[i] = rest(dg[i], gv[i], wild[i]);
+        du2[i] = rest(du[i], uv[i], wild[i]);
       }
-      __builtin_memcpy(row + 2 * Fp, dg, 16);
-      __builtin_memcpy(row + 3 * Fp, du, 16);
+      __builtin_memcpy(row + 2 * Fp, dg2, 16);
+      __builtin_memcpy(row + 3 * Fp, du2, 16);
     }
+    __builtin_memcpy(row, dg, 16);
+    __builtin_memcpy(row + Fp, du, 16);
   }
 }
 

@@ -404,3 +404,31 @@ def test_same_bits_whatever_the_memory_held(m, c, f, dtype, wdtype):
         for a, b in zip(got, first):
             assert torch.equal(a, b)
     check(x, wg, wu, dh, "swish", first)
+
+
+@pytest.mark.parametrize("act", ["swish", "sigmoid", "relu", None])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinities_of_the_gradients_are_those_of_the_formula(dtype, act):
+    """One infinity in a row, a weight or an incoming gradient: the gradients' infinities and NaN are
+    the formula's, and finite values stay finite."""
+    for where in ("x", "wg", "wu", "dh", "wg of a zero"):
+        for m in (5, 300):
+            x, wg, wu, dh = inputs(m, 64, 136, dtype, 7)
+            # away from zero, so that no rounding makes one (0 times an infinity is NaN)
+            x, wg, wu, dh = (t.sign() * (t.abs() + 2.0 ** -3) for t in (x, wg, wu, dh))
+            {"x": x, "wg": wg, "wu": wu, "dh": dh, "wg of a zero": wg}[where][3, 9] = float("inf")
+            if where == "wg of a zero":
+                x[1, 9] = 0.0
+                if act == "relu":
+                    continue          # (a gate of NaN has no side)
+            got = run(x, wg, wu, dh, act)
+            xd, gd, ud, d = (t.double().cpu() for t in (x, wg, wu, dh))
+            g, u = xd @ gd.t(), xd @ ud.t()
+            a, s = act_of(g, act)
+            dg, du = d * u * s, d * a
+            want = (a * u, dg @ gd + du @ ud, dg.t() @ xd, du.t() @ xd)
+            for name, t, w in zip(("h", "dx", "dwg", "dwu"), got, want):
+                t = t.double().cpu()
+                assert torch.equal(t.isnan(), w.isnan()), (where, m, name)
+                assert torch.equal(t[w.isinf()], w[w.isinf()]), (where, m, name)
+                assert torch.isfinite(t[torch.isfinite(w)]).all(), (where, m, name)
