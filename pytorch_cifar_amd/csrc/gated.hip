@@ -50,35 +50,36 @@ struct Mat<float> {
   }
 };
 
-// fp32 products on the bf16 matrix instruction. A float is the exact sum of three bf16, its 8 leading
-// bits, the next 8 and the last (cut off, not rounded: 8 bits each), and of the nine products of two
-// such sums the six largest are taken: what is left out is 2^-23 of a product at most. Six
-// instructions of 32 terms take 96 cycles, the eight fp32 ones 256: gated_linear of 1021 x 512 -> 1365
-// forward and backward 127 -> 104 us; 2048 x 2048 -> 5504 forward at 190 TFLOP/s, the library's fp32
-// product at 140. (Below 2^-110 the last parts leave the type's range.) An infinity has no such parts:
-// a tile that meets one is computed again by the fp32 instruction.
+// fp32 products on the bf16 matrix instruction. A float is the exact sum of three bf16: itself rounded to
+// nearest, what is left (at most 2^-8 of its power of two) rounded likewise, and the rest (2^-17). Of the
+// nine products of two such sums the six largest are taken: what is left out is 2^-24 of a product at
+// most, of either sign (parts that are cut off instead leave out 2^-21, always toward zero, for the same
+// eleven instructions a pair; the large product below runs 3 % faster on them). Six instructions of 32
+// terms take 96 cycles, the eight fp32 ones 256: gated_linear of 1021 x 512 -> 1365 forward and backward
+// 127 -> 103 us; 2048 x 2048 -> 5504 forward at 188 TFLOP/s, the library's fp32 product at 140. (Below 2^-110 the last parts leave the type's range.)
+// An infinity, and what rounds to one, has no such parts: a tile that meets one is computed again by the
+// fp32 instruction.
+constexpr float kSplitMost = 0x1.ffp127f;   // from here on
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 struct Split {
   bf16x8 h, m, l;
 };
 __device__ __forceinline__ Split split3(const f32x8& v) {
-  uint32_t a[8], b[8], c[8];
+  uint32_t w[3][4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    a[e] = __float_as_uint(v[e]);
-    const float r = v[e] - __uint_as_float(a[e] & 0xffff0000u);
-    b[e] = __float_as_uint(r);
-    c[e] = __float_as_uint(r - __uint_as_float(b[e] & 0xffff0000u));
+  for (int i = 0; i < 4; ++i) {
+    float x = v[2 * i], y = v[2 * i + 1];
+#pragma unroll
+    for (int part = 0; part < 3; ++part) {
+      const uint32_t p = pack2(x, y);
+      w[part][i] = p;
+      x -= __uint_as_float(p << 16);
+      y -= __uint_as_float(p & 0xffff0000u);
+    }
   }
-  auto high = [](const uint32_t* x) {   // the upper halves
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x07060302u);
-    bf16x8 o;
-    __builtin_memcpy(&o, w, 16);
-    return o;
-  };
-  return {high(a), high(b), high(c)};
+  Split s;
+  __builtin_memcpy(&s, w, sizeof(s));
+  return s;
 }
 constexpr int kRow = 128;   // bytes of a row that a K tile takes: 64 16-bit or 32 fp32 terms
 template <typename E>
@@ -443,7 +444,7 @@ __attribute__((amdgpu_waves_per_eu(2, 2))) void gated_kernel(GatedArgs a, int mt
     __syncthreads();
     if (threadIdx.x == 0) *met = 0;
     __syncthreads();
-    if (most == INFINITY) *met = 1;
+    if (most >= kSplitMost) *met = 1;
     __syncthreads();
     const bool again = *met != 0;
     __syncthreads();

@@ -432,3 +432,38 @@ def test_infinities_of_the_gradients_are_those_of_the_formula(dtype, act):
                 assert torch.equal(t.isnan(), w.isnan()), (where, m, name)
                 assert torch.equal(t[w.isinf()], w[w.isinf()]), (where, m, name)
                 assert torch.isfinite(t[torch.isfinite(w)]).all(), (where, m, name)
+
+
+@pytest.mark.parametrize("c", [1, 2, 3])
+@pytest.mark.parametrize("bits", [0x3f80ffff, 0x3f80feff, 0x3fff7f7f, 0x3f808080, 0x3f817fff, 0x3fffffff])
+def test_fp32_products_of_three_parts(bits, c):
+    """fp32 products are six of their operands' three bf16 parts. A projection of c equal terms: what is
+    left out is 2^-24 of each, the fp32 sum of the largest parts' products rounds c times by a step at
+    most, and the smaller parts' (2^-7 of them) sums by 2^-6 together; h is their product, rounded once."""
+    v = torch.tensor(bits, dtype=torch.int32).view(torch.float32).item()
+    for s in (1.0, -1.0):
+        x = torch.full((70, c), v, device="cuda")
+        wg, wu = torch.full((40, c), v, device="cuda"), torch.full((40, c), s * v, device="cuda")
+        h = PF.gated_linear(x, wg, wu, None)
+        want = s * (c * v * v) ** 2
+        step = 2 * (1 + 2 * c + 2.0 ** -4) + 1
+        assert ((h.double() - want).abs() <= step * U * abs(want)).all(), ((h.double() / want - 1).abs().max() / U)
+
+
+def test_fp32_operands_that_bf16_does_not_hold():
+    """Finite numbers that round to infinity in bf16."""
+    big = torch.finfo(torch.float32).max
+    x, wg, wu, dh = inputs(80, 24, 40, torch.float32, 14)
+    x[3, 5], x[4] = big, 0.0
+    wg[:, 5] = wg[:, 5].sign() * 2.0 ** -120
+    wu[:, 5] = 0.0
+    x[4, 2], wg[7, 2], wg[8] = -big, 1.0, 0.0
+    wu[:, 2] = 2.0 ** -100
+    wg[8, 2] = 2.0 ** -100
+    h = PF.gated_linear(x, wg, wu, None)
+    g, u = x.double() @ wg.double().t(), x.double() @ wu.double().t()
+    want = g * u
+    mag = (x.double().abs() @ wg.double().abs().t()) * u.abs() + g.abs() * (x.double().abs() @ wu.double().abs().t())
+    fine = want.abs() < 2.0 ** 127
+    assert ((h.double() - want).abs() <= 64 * U * mag)[fine].all()
+    assert h.isnan().sum() == 0
