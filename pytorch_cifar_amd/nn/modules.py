@@ -92,11 +92,13 @@ class GatedLinear(nn.Module):
     """act(x Wg^T) * (x Wu^T): the widening half of a gated feed-forward block (a ``Linear`` back to
     the width follows it). fp32 parameters ``weight_gate`` and ``weight_up`` [hidden_features,
     in_features], initialised as ``Linear`` does; rows are [..., in_features] or the pixels of an
-    NCHW-shaped feature map, in the type they come in (the weights are rounded to it)."""
+    NCHW-shaped feature map (``dim`` as in ``gated_linear``), in the type they come in (the weights are
+    rounded to it)."""
 
-    def __init__(self, in_features, hidden_features, act="swish"):
+    def __init__(self, in_features, hidden_features, act="swish", dim=None):
         super().__init__()
         self.in_features, self.hidden_features, self.act = in_features, hidden_features, act
+        self.dim = dim
         self.weight_gate = nn.Parameter(torch.empty(hidden_features, in_features))
         self.weight_up = nn.Parameter(torch.empty(hidden_features, in_features))
         bound = OF.kaiming_fan_in_bound(in_features)
@@ -104,10 +106,11 @@ class GatedLinear(nn.Module):
             nn.init.uniform_(w, -bound, bound)
 
     def forward(self, x):
-        return gated_linear(x, self.weight_gate, self.weight_up, self.act)
+        return gated_linear(x, self.weight_gate, self.weight_up, self.act, self.dim)
 
     def extra_repr(self):
-        return f"{self.in_features}, {self.hidden_features}, act={self.act!r}"
+        return (f"{self.in_features}, {self.hidden_features}, act={self.act!r}"
+                + (f", dim={self.dim}" if self.dim is not None else ""))
 
 
 class ReLU(nn.ReLU):

@@ -13,11 +13,13 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 MAX_WIDTH = 1 << 19
 
 
-def gated_linear(x, w_gate, w_up, act="swish"):
+def gated_linear(x, w_gate, w_up, act="swish", dim=None):
     """``act(x @ w_gate.T) * (x @ w_up.T)`` with ``w_gate``, ``w_up`` [hidden, width].
 
-    ``x`` is [..., width], or an NCHW-shaped feature map [N, width, H, W], whose pixels are the rows;
-    the result has ``hidden`` in the place of ``width``. ``act``: "swish" ("silu"), "sigmoid",
+    ``x`` is [..., width]; with four dimensions it is taken for an NCHW-shaped feature map [N, width, H,
+    W], whose pixels are the rows. ``dim`` says which: -1 rows of any shape ([batch, heads, tokens,
+    width]), 1 a feature map. It has to where dimensions 1 and 3 are both as long as the width. The result
+    has ``hidden`` in the place of ``width``. ``act``: "swish" ("silu"), "sigmoid",
     "relu" or None. fp32, bf16 and fp16 rows; the weights have the rows' type, or are fp32 masters,
     which are rounded to it and whose gradients are fp32. Sums are fp32; in 16 bits the gradients of
     the projections are rounded once to the rows' type, the operand of the products that follow (small
@@ -28,7 +30,15 @@ def gated_linear(x, w_gate, w_up, act="swish"):
     """
     if act not in ACT:
         raise ValueError(f"act must be one of {sorted(a for a in ACT if a)} or None, got {act!r}")
-    if x.dim() == 4:
+    if dim not in (None, 1, -1):
+        raise ValueError(f"dim must be 1 (a feature map), -1 (rows) or None, got {dim!r}")
+    if dim == 1 and x.dim() != 4:
+        raise ValueError(f"dim=1 is that of a feature map [N, width, H, W], x is {tuple(x.shape)}")
+    if x.dim() == 4 and dim != -1:
+        if w_gate.dim() == 2 and dim is None and x.shape[3] == w_gate.shape[1]:
+            raise ValueError(f"x {tuple(x.shape)} ends with the weights' width {x.shape[3]}"
+                             + (", and dimension 1 is as long: dim must be 1 or -1" if x.shape[1] == x.shape[3]
+                                else ", but four dimensions are a feature map unless dim=-1"))
         y = gated_linear(x.permute(0, 2, 3, 1).unsqueeze(0), w_gate, w_up, act)[0]
         return y.permute(0, 3, 1, 2)
     if not _ref(x):

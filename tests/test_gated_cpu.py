@@ -83,3 +83,31 @@ W = torch.zeros(9, 7)
 def test_refusals(args, err):
     with pytest.raises(err):
         PF.gated_linear(*args)
+
+
+def test_rows_of_four_dimensions():
+    """[batch, heads, tokens, width] beside feature maps: `dim` says which, and nothing is guessed."""
+    torch.manual_seed(0)
+    wg, wu = torch.randn(5, 7), torch.randn(5, 7)
+
+    def check(h, rows):
+        g, u = rows.double() @ wg.double().t(), rows.double() @ wu.double().t()
+        dg, du = ((rows.double().abs() @ w.double().abs().t()) * 8 * U for w in (wg, wu))
+        a = ACTS["swish"](g)
+        tol = 1.1 * dg * u.abs() + a.abs() * du + dg * du + 8 * U * (a * u).abs()
+        assert h.shape == (*rows.shape[:-1], 5) and ((h.double() - a * u).abs() <= tol).all()
+
+    for shape in ((2, 3, 4, 7), (2, 7, 3, 7)):
+        x = torch.randn(*shape)
+        check(PF.gated_linear(x, wg, wu, dim=-1), x)
+        m = pnn.GatedLinear(7, 5, dim=-1)
+        m.load_state_dict({"weight_gate": wg, "weight_up": wu})
+        check(m(x).detach(), x)
+        assert "dim=-1" in repr(m)
+        with pytest.raises(ValueError, match="dim"):
+            PF.gated_linear(x, wg, wu)
+    for x in (torch.randn(2, 7, 3, 7), torch.randn(2, 7, 3, 4)):
+        check(PF.gated_linear(x, wg, wu, dim=1).permute(0, 2, 3, 1), x.permute(0, 2, 3, 1))
+    for dim, x in ((0, x), (3, x), (1, x[0]), (1, torch.randn(2, 3, 4, 7))):
+        with pytest.raises(ValueError):
+            PF.gated_linear(x, wg, wu, dim=dim)

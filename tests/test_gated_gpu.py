@@ -467,3 +467,16 @@ def test_fp32_operands_that_bf16_does_not_hold():
     fine = want.abs() < 2.0 ** 127
     assert ((h.double() - want).abs() <= 64 * U * mag)[fine].all()
     assert h.isnan().sum() == 0
+
+
+def test_rows_of_four_dimensions():
+    x, wg, wu, dh = inputs(24, 16, 40, torch.bfloat16, 15)
+    base = run(x, wg, wu, dh, "swish")
+    for shape in ((2, 3, 4), (1, 16, 1), (2, 12, 1)):
+        n = shape[0] * shape[1] * shape[2]
+        leaves = [t.detach().requires_grad_(True) for t in (x[:n].view(*shape, 16), wg, wu)]
+        h = PF.gated_linear(*leaves, dim=-1)
+        (dx,) = torch.autograd.grad(h, leaves[:1], dh[:n].view(*shape, 40))
+        assert torch.equal(h.view(n, 40), base[0][:n]) and torch.equal(dx.view(n, 16), base[1][:n])
+        with pytest.raises(ValueError, match="dim"):
+            PF.gated_linear(*leaves)
