@@ -191,6 +191,7 @@ Tensor distill_loss(const Tensor& logits, const Tensor& values, const Tensor& in
                     bool debug) {
   check_logits(logits);
   check_temp(temperature);
+  no_tangent(logits, "distill_loss");
   Loss l{temperature, alpha, tail,
          reduction == "none" ? 0 : reduction == "mean" ? 1 : reduction == "sum" ? 2 : -1,
          ignore_index};
@@ -213,6 +214,7 @@ Tensor distill_loss(const Tensor& logits, const Tensor& values, const Tensor& in
     PCA_VALUE(t.device() == logits.device(), name, " is on ", t.device(), ", the logits are on ",
               logits.device());
     PCA_VALUE(!t.requires_grad(), name, " requires grad: a teacher's answer is data, detach it");
+    no_tangent(t, "distill_loss");
     return t.contiguous();
   };
   c10::OptionalDeviceGuard guard(at::device_of(logits));

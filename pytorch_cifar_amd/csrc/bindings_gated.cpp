@@ -196,6 +196,7 @@ Tensor gated_linear(const Tensor& x, const Tensor& wg, const Tensor& wu, int64_t
   PCA_VALUE(wg.device() == x.device() && wu.device() == x.device(), "weights are on ", wg.device(),
             " and ", wu.device(), ", x is on ", x.device());
   PCA_VALUE(x.numel() / x.size(-1) <= (int64_t(1) << 30), "x has more than 2^30 rows");
+  for (const Tensor* t : {&x, &wg, &wu}) no_tangent(*t, "gated_linear");
   PCA_VALUE(act >= ACT_NONE && act <= ACT_SIGMOID, "activation");
   c10::OptionalDeviceGuard guard(at::device_of(x));
   Tensor h;

@@ -34,6 +34,13 @@ inline void once_differentiable(std::vector<at::Tensor>& grads, const char* what
     }
 }
 
+// No node here has a forward-mode derivative, and a dual tensor need not require grad: refused, never a
+// result without its tangent.
+inline void no_tangent(const at::Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), what,
+                              " has no forward-mode derivative");
+}
+
 // debug mode: an asynchronous fault or launch error is raised at the operator that caused it
 inline void debug_check(bool debug, const char* what) {
   if (!debug) return;

@@ -12,6 +12,7 @@ from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from .. import _native
 from .functional import _C, _ref
@@ -65,7 +66,8 @@ def top_logits(logits, k, temperature=1.0):
 
     Descending; among equal logits the lowest class comes first, and NaN counts as the largest.
     ``lse`` is taken at ``temperature``, that of the loss that will use it; the values are the
-    logits as they are. Not differentiable: a teacher's answer is data to its student.
+    logits as they are. Not differentiable, backward or forward: a teacher's answer is data to its
+    student.
     """
     if not _ref(logits):
         return TopLogits(*_C().top_logits(logits, k, temperature))
@@ -76,6 +78,7 @@ def top_logits(logits, k, temperature=1.0):
     if not 1 <= k <= min(n, MAX_K):
         raise ValueError(f"k must be 1 to {min(n, MAX_K)}, got {k}")
     with torch.no_grad():
+        logits = forward_ad.unpack_dual(logits).primal
         z = logits.float()
         values, indices = torch.sort(z, dim=-1, descending=True, stable=True)
         lse = torch.logsumexp(z.double() / t, -1).float()
@@ -151,7 +154,7 @@ def distill_loss(logits, top, target=None, temperature=1.0, alpha=None, tail=Fal
     loss and gradient 0. ``reduction``: "mean" over all rows, "sum", or "none". A class outside
     the row makes its loss and gradient NaN.
 
-    Teacher's side is data: gradients flow to ``logits`` alone. Forward and backward can be captured,
+    Teacher's side is data: gradients flow to ``logits`` alone, once and in reverse mode. Forward and backward can be captured,
     together or apart. As with every autograd function, no eager graph of the same leaves may be alive
     while a backward is captured.
     """

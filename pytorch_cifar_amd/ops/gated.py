@@ -25,8 +25,8 @@ def gated_linear(x, w_gate, w_up, act="swish", dim=None):
     the projections are rounded once to the rows' type, the operand of the products that follow (small
     layers keep them in two parts). In fp16 what overflows there is an infinity.
 
-    Forward and backward can be captured, together or apart. As with every autograd function, no eager
-    graph of the same leaves may be alive while a backward is captured.
+    Differentiable once, in reverse mode. Forward and backward can be captured, together or apart. As with
+    every autograd function, no eager graph of the same leaves may be alive while a backward is captured.
     """
     if act not in ACT:
         raise ValueError(f"act must be one of {sorted(a for a in ACT if a)} or None, got {act!r}")

@@ -211,3 +211,20 @@ def test_gradient_of_the_rest_under_a_mask():
     want = torch.full((300,), -rest / 299, dtype=torch.float64)
     want[5] = rest                          # (q = 1 there, and p = 1 - rest)
     assert ((z.grad[0].double() - want).abs() <= 2 * HALF * want.abs()).all()
+
+
+def test_a_teachers_answer_has_no_tangent():
+    from torch.autograd import forward_ad as fa
+
+    z, top, y, _ = case()
+    with fa.dual_level():
+        dual = fa.make_dual(z, torch.ones_like(z) * torch.arange(z.shape[1]))
+        assert fa.unpack_dual(PF.top_logits(dual, 3).values).tangent is None
+        assert fa.unpack_dual(PF.top_logits(dual, 3).lse).tangent is None
+        # the loss's is that of its gradient
+        out = fa.unpack_dual(PF.distill_loss(dual, top, y, temperature=2.0, alpha=0.5, tail=True))
+    x = z.clone().requires_grad_(True)
+    PF.distill_loss(x, top, y, temperature=2.0, alpha=0.5, tail=True).backward()
+    want = (x.grad.double() * torch.arange(z.shape[1])).sum().item()
+    # 91 elements rounded to fp32, times 12 at most, and the sum rounded
+    assert abs(out.tangent.item() - want) <= HALF * (12 * x.grad.double().abs().sum().item() + abs(want))

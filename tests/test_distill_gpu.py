@@ -689,3 +689,24 @@ def test_classes_masked_by_some_millions(v, t):
         assert ((loss.cpu().double() - want).abs() <= tl + 2 * U * want.abs()).all()
         assert ((x.grad.cpu().double() - grad).abs()[:, v - 40:] <= tg(torch.float32)).all()
         assert not x.grad[:, :v - 40].any()
+
+
+def test_forward_mode_is_refused():
+    from torch.autograd import forward_ad as fa
+
+    z, top, y = distill_inputs(4, 50, 3, torch.float32, 1.0)
+    z, top = z.cuda(), gpu_top(top)
+    with fa.dual_level():
+        for leaf in (z, z.clone().requires_grad_(True)):
+            dual = fa.make_dual(leaf, torch.ones_like(leaf))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                PF.distill_loss(dual, top)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                PF.distill_loss(dual[:2, 1:40], PF.TopLogits(*(a[:2] for a in top)))
+        values = fa.make_dual(top.values, torch.ones_like(top.values))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            PF.distill_loss(z, PF.TopLogits(values, top.indices, top.lse))
+        # data, as in reverse mode
+        assert fa.unpack_dual(PF.top_logits(fa.make_dual(z, torch.ones_like(z)), 3).values).tangent is None
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: PF.distill_loss(x, top), (z,), (torch.ones_like(z),))

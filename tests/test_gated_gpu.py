@@ -480,3 +480,18 @@ def test_rows_of_four_dimensions():
         assert torch.equal(h.view(n, 40), base[0][:n]) and torch.equal(dx.view(n, 16), base[1][:n])
         with pytest.raises(ValueError, match="dim"):
             PF.gated_linear(*leaves)
+
+
+def test_forward_mode_is_refused():
+    from torch.autograd import forward_ad as fa
+
+    args = inputs(8, 16, 24, torch.bfloat16, 16)[:3]
+    with fa.dual_level():
+        for i in range(3):
+            for leaf in (args[i], args[i].clone().requires_grad_(True)):
+                mixed = list(args)
+                mixed[i] = fa.make_dual(leaf, torch.ones_like(leaf))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    PF.gated_linear(*mixed)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: PF.gated_linear(x, *args[1:]), (args[0],), (torch.ones_like(args[0]),))
