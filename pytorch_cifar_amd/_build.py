@@ -3,7 +3,8 @@
 No hipify, no torch JIT cache: every ``csrc/*.hip`` kernel file and ``csrc/*.cpp`` host file is
 compiled explicitly with ``hipcc --offload-arch=gfx950`` into ``build/obj`` and linked into an
 extension module that lives next to this file, so the built ``.so`` travels with the repository
-snapshot to the GPU box.  Objects are rebuilt only when a source or header is newer.
+snapshot to the GPU box.  Objects are rebuilt only when a source or header is newer or the command that
+compiles them is another.
 
 Usage:  python -m pytorch_cifar_amd._build [--force] [-v]
 """
@@ -52,23 +53,28 @@ def _torch_paths():
     return incs, libdir, abi
 
 
+# what every compile has, wherever torch and Python are installed
+FLAGS = [
+    "-O3",
+    "-std=c++17",
+    "-fPIC",
+    "-DUSE_ROCM",
+    "-D__HIP_PLATFORM_AMD__=1",
+    f"-DTORCH_EXTENSION_NAME={EXT_NAME}",
+    "-DTORCH_API_INCLUDE_EXTENSION_H",
+    "-Wno-unused-result",
+    "-Wno-deprecated-declarations",
+    "-Wno-unused-command-line-argument",
+]
+
+
+def _device_flags():
+    return ["-x", "hip", f"--offload-arch={ARCH}", *NO_PACKED_FP32]
+
+
 def _common_flags(incs, abi):
     py_inc = sysconfig.get_paths()["include"]
-    flags = [
-        "-O3",
-        "-std=c++17",
-        "-fPIC",
-        "-DUSE_ROCM",
-        "-D__HIP_PLATFORM_AMD__=1",
-        f"-DTORCH_EXTENSION_NAME={EXT_NAME}",
-        "-DTORCH_API_INCLUDE_EXTENSION_H",
-        f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-        "-Wno-unused-result",
-        "-Wno-deprecated-declarations",
-        "-Wno-unused-command-line-argument",
-        f"-I{CSRC}",
-        f"-I{py_inc}",
-    ]
+    flags = [*FLAGS, f"-D_GLIBCXX_USE_CXX11_ABI={abi}", f"-I{CSRC}", f"-I{py_inc}"]
     # build-time kernel variants for same-box A/B trees (e.g. -DPCA_IGEMM_DMA_SPREAD=1)
     flags += os.environ.get("PCA_EXTRA_HIPCC_FLAGS", "").split()
     flags += [f"-I{p}" for p in incs]
@@ -76,10 +82,12 @@ def _common_flags(incs, abi):
 
 
 def source_digest() -> str:
-    """sha256 over every csrc source/header (name + bytes): identifies what a built .so is of."""
+    """sha256 over every csrc source/header (name + bytes) and the flags they are compiled with:
+    identifies what a built .so is of. (Not over PCA_EXTRA_HIPCC_FLAGS: a variant that was built with
+    some runs where they are not set.)"""
     import hashlib
 
-    h = hashlib.sha256()
+    h = hashlib.sha256(repr((FLAGS, _device_flags())).encode())
     for f in sorted(os.listdir(CSRC)):
         if f.endswith((".hip", ".cpp", ".h")):
             h.update(f.encode())
@@ -93,7 +101,7 @@ def digest_path() -> str:
 
 
 def is_stale():
-    """True when the in-tree .so is missing or was built from different csrc contents, False when
+    """True when the in-tree .so is missing or was built from different csrc contents or flags, False when
     its recorded digest matches, None when unknown (the .so exists but its git-ignored ``.srchash``
     does not, e.g. a fresh checkout next to a shipped .so): the loader then compares the digest the
     .so carries itself (``_C.src_digest()``) after import."""
@@ -118,23 +126,33 @@ def _headers():
     return [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
 
 
-def _needs_build(src: str, obj: str, deps) -> bool:
-    if not os.path.exists(obj):
+def _command(src, obj, flags):
+    return [_hipcc(), *flags, *(_device_flags() if src.endswith(".hip") else []), "-c", src, "-o", obj]
+
+
+def _needs_build(src: str, obj: str, deps, flags) -> bool:
+    try:
+        t = os.path.getmtime(obj)
+        with open(obj + ".cmd") as fh:
+            if fh.read() != repr(_command(src, obj, flags)):
+                return True
+    except OSError:
         return True
-    t = os.path.getmtime(obj)
     return any(os.path.getmtime(d) > t for d in [src, *deps])
 
 
 def _compile(src, obj, flags, verbose):
-    cmd = [_hipcc()] + flags
-    if src.endswith(".hip"):
-        cmd += ["-x", "hip", f"--offload-arch={ARCH}", *NO_PACKED_FP32]
-    cmd += ["-c", src, "-o", obj]
+    cmd = _command(src, obj, flags)
+    stamp = obj + ".cmd"      # the command that made the object, written once it has
+    if os.path.exists(stamp):
+        os.remove(stamp)
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"hipcc failed for {os.path.basename(src)}:\n{r.stderr[-6000:]}")
+    with open(stamp, "w") as fh:
+        fh.write(repr(cmd))
     return obj
 
 
@@ -151,7 +169,7 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -
     for s in srcs:
         o = os.path.join(OBJ_DIR, os.path.basename(s) + ".o")
         objs.append(o)
-        if force or _needs_build(s, o, hdrs):
+        if force or _needs_build(s, o, hdrs, flags):
             todo.append((s, o))
     jobs = jobs or min(len(todo) or 1, int(os.environ.get("MAX_JOBS", os.cpu_count() or 4)), 8)
     if todo:
