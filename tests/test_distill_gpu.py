@@ -710,3 +710,91 @@ def test_forward_mode_is_refused():
         assert fa.unpack_dual(PF.top_logits(fa.make_dual(z, torch.ones_like(z)), 3).values).tangent is None
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda x: PF.distill_loss(x, top), (z,), (torch.ones_like(z),))
+
+
+def check_streamed(z, t, terms, x_loss, want, x_grad, grad, alpha, seeds):
+    """Losses and gradients on the GPU, where a thread sums `terms` terms of a row."""
+    c = (3 * spread(z, t) + terms + 4) * U
+    assert ((x_loss.double() - want).abs() <= 2 * c * (alpha * t * t + 1 - alpha) + 2 * U * want.abs()).all()
+    if x_grad is None:
+        return
+    q = alpha * t * torch.softmax(z.double() / t, 1) + (1 - alpha) * torch.softmax(z.double(), 1)
+    tol = 2 * c * (q * seeds.double()[:, None] + grad.abs()) + torch.finfo(z.dtype).eps / 2 * grad.abs()
+    tol += 2.0 ** -25 if z.dtype == torch.float16 else 1e-37
+    assert ((x_grad.double() - grad).abs() <= tol).all()
+
+
+# rows and chunks of 16 bytes: streamed by 256, 512 or 1024 threads with a gradient and without (a row of
+# up to 8192 chunks takes fewer threads than a longer one, and few rows take more)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("r, chunks", [(530, 1030), (530, 8190), (530, 8300), (1030, 1251), (1030, 8190), (1030, 8193),
+                                       (1100, 2500), (300, 1500)])
+def test_distill_streamed_by_few_threads(r, chunks, dtype):
+    if dtype == torch.float32:
+        v = chunks * 4 - 3
+    else:
+        v = chunks * 8 - 5
+    t, alpha, k = 2.0, 0.7, 33
+    g = torch.Generator(device="cuda").manual_seed(r + chunks)
+    teacher = (3 * torch.randn(r, v, generator=g, device="cuda")).to(dtype)
+    z = (0.6 * teacher.float() + 1.5 * torch.randn(r, v, generator=g, device="cuda")).to(dtype)
+    top = PF.top_logits(teacher, k, t)
+    del teacher
+    y = torch.randint(0, v, (r,), generator=g, device="cuda")
+    top.indices[3, 7:] = -1
+    top.indices[5] = -1
+    top.indices[6, 3] = top.indices[6, 1]
+    y[7::50] = -100
+    seeds = torch.rand(r, generator=g, device="cuda") + 0.5
+    terms = (chunks + 255) // 256 * (4 if dtype == torch.float32 else 8)      # (256 threads: the most)
+    for tail in (True, False):
+        kw = dict(temperature=t, alpha=alpha, tail=tail, reduction="none")
+        x = z.detach().requires_grad_(True)
+        loss = PF.distill_loss(x, top, y, **kw)
+        (got,) = torch.autograd.grad(loss, x, seeds)
+        alone = PF.distill_loss(z, top, y, **kw)
+        for at in range(0, r, 265):               # (64 bits of some rows at a time)
+            s = slice(at, min(at + 265, r))
+            part = PF.TopLogits(*(a[s] for a in top))
+            want, grad = oracle_on_gpu(z[s], part, y[s], t, alpha, tail, seeds[s])
+            check_streamed(z[s], t, terms, loss.detach()[s], want, got[s], grad, alpha, seeds[s])
+            check_streamed(z[s], t, terms, alone[s], want, None, None, alpha, seeds[s])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("r, chunks, k", [(520, 1030, 5), (520, 1251, 120), (520, 8192, 256), (520, 8193, 256), (300, 2000, 100),
+                                          (520, 16384, 384), (520, 16385, 300), (300, 6000, 640), (300, 4000, 700),
+                                          (300, 1100, 1024), (200, 3000, 200)])
+def test_top_logits_streamed_by_few_threads(r, chunks, k, dtype):
+    v = chunks * 4 - 3 if dtype == torch.float32 else chunks * 8 - 5
+    g = torch.Generator(device="cuda").manual_seed(r + chunks)
+    z = (3 * torch.randn(r, v, generator=g, device="cuda")).to(dtype)
+    z[1] = z[1].sort()[0]
+    z[2] = z[2].sort(descending=True)[0]
+    z[3, v // 3:] = -math.inf
+    z[4, :v // 2] = torch.finfo(dtype).min
+    z[5] = z[5].float().round().to(dtype)
+    z[6, v // 2] = math.nan
+    z[7] = 1.0
+    top = PF.top_logits(z, k, 2.0)
+    some = list(range(9)) + [r // 2, r - 2, r - 1]
+    want = PF.top_logits(z[some].cpu(), k, 2.0)
+    assert torch.equal(top.indices[some].cpu(), want.indices)
+    # all rows: descending, each value where it says, no class twice, nothing left out above the last
+    for at in range(0, r, 130):
+        s = slice(at, min(at + 130, r))
+        f = torch.nan_to_num(z[s].float(), nan=math.inf)
+        vals = f.gather(1, top.indices[s].long())
+        assert torch.equal(vals, torch.nan_to_num(top.values[s].float(), nan=math.inf))
+        assert (vals[:, :-1] >= vals[:, 1:]).all()
+        order = top.indices[s].sort(1)[0]
+        assert (order[:, 1:] > order[:, :-1]).all()
+        assert ((f > vals[:, -1:]).sum(1) < k).all()
+        keep = torch.tensor([i for i in range(at, s.stop) if i != 6], device="cuda") - at
+        # C of a thread's most terms (256 threads)
+        terms = (chunks + 255) // 256 * (4 if dtype == torch.float32 else 8)
+        rows = z[s][keep]
+        c = (3 * spread(rows.masked_fill(rows <= torch.finfo(dtype).min, 0), 2.0) + terms + 4) * U
+        ref = torch.logsumexp(rows.double() / 2.0, 1)
+        assert ((top.lse[s][keep].double() - ref).abs() <= c + U * ref.abs()).all()
+    assert top.lse[6].isnan()
