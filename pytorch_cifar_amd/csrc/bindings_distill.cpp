@@ -33,8 +33,10 @@ void check_logits(const Tensor& z) {
   PCA_VALUE(z.numel() / z.size(-1) < (int64_t(1) << 31), "logits has too many rows");
 }
 
+// (log2 e / T is an fp32 number)
 void check_temp(double t) {
-  PCA_VALUE(std::isfinite(t) && t > 0, "temperature must be positive and finite, got ", t);
+  PCA_VALUE(t >= kDistillMinTemp && t <= 1 / kDistillMinTemp,
+            "temperature must be positive, 2^-64 to 2^64, got ", t);
 }
 
 // shape with the last dimension replaced by k (dropped for k = 0)

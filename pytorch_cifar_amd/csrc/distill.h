@@ -6,6 +6,7 @@ namespace pca {
 
 constexpr int kDistillMaxClasses = 1 << 18;   // classes of a row (the kept-class map is 32 KiB)
 constexpr int kDistillMaxK = 1024;            // kept logits of a row
+constexpr double kDistillMinTemp = 5.421010862427522e-20;   // 2^-64
 constexpr double kDistillRest = 1.0 / (1 << 20);
 
 enum LogitType : int { LOGIT_F32 = 0, LOGIT_BF16 = 1, LOGIT_F16 = 2 };

@@ -19,6 +19,7 @@ from .functional import _C, _ref
 
 MAX_CLASSES = 1 << 18
 MAX_K = 1024
+MIN_TEMPERATURE = 2.0 ** -64     # csrc/distill.h kDistillMinTemp; its reciprocal is the largest
 REST = 2.0 ** -20        # csrc/distill.h kDistillRest
 _REDUCTION = ("none", "mean", "sum")
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
@@ -44,8 +45,8 @@ def _check_logits(logits, name="logits"):
 
 def _check_temperature(t):
     t = float(t)
-    if not (math.isfinite(t) and t > 0):
-        raise ValueError(f"temperature must be positive and finite, got {t}")
+    if not MIN_TEMPERATURE <= t <= 1 / MIN_TEMPERATURE:
+        raise ValueError(f"temperature must be positive, 2^-64 to 2^64, got {t}")
     return t
 
 

@@ -228,3 +228,12 @@ def test_a_teachers_answer_has_no_tangent():
     want = (x.grad.double() * torch.arange(z.shape[1])).sum().item()
     # 91 elements rounded to fp32, times 12 at most, and the sum rounded
     assert abs(out.tangent.item() - want) <= HALF * (12 * x.grad.double().abs().sum().item() + abs(want))
+
+
+@pytest.mark.parametrize("t", [2.0 ** -65, 2.0 ** 65, 1e-300, 1e300, math.nan])
+def test_temperatures_out_of_range(t):
+    z, top, _, teacher = case()
+    with pytest.raises(ValueError, match="temperature"):
+        PF.top_logits(teacher, 3, t)
+    with pytest.raises(ValueError, match="temperature"):
+        PF.distill_loss(z, top, temperature=t)

@@ -798,3 +798,19 @@ def test_top_logits_streamed_by_few_threads(r, chunks, k, dtype):
         ref = torch.logsumexp(rows.double() / 2.0, 1)
         assert ((top.lse[s][keep].double() - ref).abs() <= c + U * ref.abs()).all()
     assert top.lse[6].isnan()
+
+
+def test_temperatures_at_the_ends_of_their_range():
+    for t in (2.0 ** -64, 2.0 ** 64):
+        z, top, y = distill_inputs(4, 50, 3, torch.float32, 1.0)
+        z.mul_(t)
+        teacher = make(4, 50, torch.float32, 3) * t
+        top = PF.top_logits(teacher, 3, t)
+        got = PF.top_logits(teacher.cuda(), 3, t)
+        assert torch.equal(got.indices.cpu(), top.indices)
+        assert ((got.lse.cpu() - top.lse).abs() <= 300 * U * top.lse.abs()).all()
+    for t in (2.0 ** -65, 2.0 ** 65, 1e-40, 1e-300, 1e300):
+        with pytest.raises(ValueError):
+            PF.top_logits(z.cuda(), 3, t)
+        with pytest.raises(ValueError):
+            PF.distill_loss(z.cuda(), gpu_top(top), temperature=t)
