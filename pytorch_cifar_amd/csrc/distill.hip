@@ -195,12 +195,15 @@ __device__ __forceinline__ A block_fold(A v, A* red, Op op) {
 }
 
 // Sum of 2^(x - base) over a thread's x = z c, in one pass without the maximum: a term costs one
-// multiply-add, the exponential and the add. The base is the first chunk's largest x, as a whole
-// number: sums of different bases are joined by exact powers of two, which meet the sum before it is
-// rounded (a thread's may be 2^127 above its base, and the base more than that below the row's: 2^-130 as
-// a factor would be zero). 2^60 above and all below it is room for what follows. A row that leaves it (a
-// first chunk of masked classes, |x| past 2^22, infinities, NaN) is summed again against its maximum
-// (`plain` below).
+// multiply-add, the exponential and the add. The base is the first chunk's largest x, as a whole number:
+// sums of different bases are joined by exact powers of two, which meet the sum before it is rounded (a
+// thread's may be 2^127 above its base, and the base more than that below the row's: 2^-130 as a factor
+// would be zero). 2^60 above and all below it is room for what follows. A row that leaves it (a first
+// chunk of masked classes, |x| past 2^22, infinities, NaN) is summed again against its maximum (`plain`
+// below).
+//
+// x - base is rounded to 24 bits, and c = log2(e) / T is one fp32 number: together a term is off by some
+// |x - base| 2^-24 relative, the row's largest too, whose distance from its maximum would be exact.
 constexpr float kNoBase = -4194304.f, kFar = 4194304.f;
 constexpr double kMost = 1152921504606846976.0;   // 2^60
 
@@ -608,7 +611,7 @@ __global__ __launch_bounds__(256) void top_small_kernel(const T* __restrict__ z,
 // a row names twice: its entries are then gathered for each of them.
 //
 // Bound by the read and the write of a row; the read for the gradient finds it in registers or in the
-// cache behind the L2s. 4096 x 128000 bf16, k 64, with rest and labels, 475 us (4.4 TB/s of 2.1 GB);
+// cache behind the L2s. 4096 x 128000 bf16, k 64, with rest and labels, 480 us (4.4 TB/s of 2.1 GB);
 // the loss alone of 2000 x 50257 fp16 50 us (4.0 TB/s).
 //
 // The loss's own gradient multiplies a row's in fp32 and 64 bits, before its one rounding: under a loss

@@ -56,9 +56,9 @@ struct Mat<float> {
 // most, of either sign (parts that are cut off instead leave out 2^-21, always toward zero, for the same
 // eleven instructions a pair; the large product below runs 3 % faster on them). Six instructions of 32
 // terms take 96 cycles, the eight fp32 ones 256: gated_linear of 1021 x 512 -> 1365 forward and backward
-// 127 -> 103 us; 2048 x 2048 -> 5504 forward at 188 TFLOP/s, the library's fp32 product at 140. (Below 2^-110 the last parts leave the type's range.)
-// An infinity, and what rounds to one, has no such parts: a tile that meets one is computed again by the
-// fp32 instruction.
+// 127 -> 103 us; 2048 x 2048 -> 5504 forward at 188 TFLOP/s, the library's fp32 product at 140. (Below
+// 2^-110 the last parts leave the type's range.) An infinity, and what rounds to one, has no such parts: a
+// tile that meets one is computed again by the fp32 instruction.
 constexpr float kSplitMost = 0x1.ffp127f;   // from here on
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 struct Split {
@@ -125,7 +125,8 @@ __device__ __forceinline__ typename Mat<E>::frag frag_terms(const char* lds, int
 }
 
 // The reciprocal instruction (1 step) in the place of the quotient, ten instructions: the epilogue
-// takes a sigmoid of every hidden unit while the matrix cores stand still.
+// takes a sigmoid of every hidden unit while the matrix cores stand still. The exponent is one rounded
+// product with a rounded constant: for negative x the result is off by some (1.25 |x| + 2) 2^-24 relative.
 __device__ __forceinline__ float sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504f));
 }
