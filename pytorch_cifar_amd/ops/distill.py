@@ -86,6 +86,11 @@ def top_logits(logits, k, temperature=1.0):
         return TopLogits(values[..., :k].to(logits.dtype), indices[..., :k].to(torch.int32), lse)
 
 
+def _finite_max(x):
+    m = x.detach().amax(1, keepdim=True)
+    return torch.where(torch.isfinite(m), m, torch.zeros_like(m))
+
+
 def _ref_distill(z, values, indices, lse, target, t, alpha, tail, ignore_index):
     """The rows' losses in 64 bits, differentiable in ``z`` [rows, classes]."""
     z = z.double()
@@ -117,13 +122,13 @@ def _ref_distill(z, values, indices, lse, target, t, alpha, tail, ignore_index):
         rest = 1.0 - p.sum(1)
         rest = torch.where(has & ~inside.all(1) & ~(rest < REST), rest, torch.zeros_like(rest))
         some = rest != 0
-        outer = logq.masked_fill(inside, -math.inf)
-        outer = torch.where(some[:, None], outer, torch.zeros_like(outer))
-        # (the logarithm of the sum apart from its base: where all other classes are masked by the type's
-        # lowest value it is below the base's last bit, and their shares with it)
-        shift = outer.detach().amax(1, keepdim=True)
-        shift = torch.where(torch.isfinite(shift), shift, torch.zeros_like(shift))
-        lrest = (outer - shift).exp().sum(1).log() + shift[:, 0]
+        zt = z / t
+        outer = torch.where(some[:, None], zt.masked_fill(inside, -math.inf), torch.zeros_like(zt))
+        # (logarithms of sums apart from their bases: where the classes not kept stand as far from the others
+        # as the type's lowest value, they are below the distance's last bit, and the shares with them)
+        top_z, top_outer = _finite_max(zt), _finite_max(outer)
+        lrest = ((outer - top_outer).exp().sum(1).log() - (zt - top_z).exp().sum(1).log()
+                 + (top_outer - top_z)[:, 0])
         loss = loss + torch.where(some, rest * (torch.where(some, rest, torch.ones_like(rest)).log()
                                                 - lrest), torch.zeros_like(rest))
     loss = torch.where(has, loss * (alpha * t * t), torch.zeros_like(loss))

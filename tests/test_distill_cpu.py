@@ -213,6 +213,21 @@ def test_gradient_of_the_rest_under_a_mask():
     assert ((z.grad[0].double() - want).abs() <= 2 * HALF * want.abs()).all()
 
 
+def test_gradient_of_the_rest_below_a_huge_logit():
+    """The kept class at half of the type's largest number: the others share the rest by their own softmax."""
+    z = torch.randn(1, 300, generator=torch.Generator().manual_seed(1))
+    z[0, 5] = torch.finfo(torch.float32).max / 2
+    top = PF.TopLogits(torch.zeros(1, 1), torch.full((1, 1), 5, dtype=torch.int32), torch.full((1,), 0.01))
+    z.requires_grad_(True)
+    PF.distill_loss(z, top, tail=True).backward()
+    rest = 1 - math.exp(-top.lse.item())
+    others = z.detach().double()[0]
+    others[5] = -math.inf
+    want = -rest * torch.softmax(others, 0)
+    want[5] = rest
+    assert ((z.grad[0].double() - want).abs() <= 2 * HALF * want.abs()).all()
+
+
 def test_a_teachers_answer_has_no_tangent():
     from torch.autograd import forward_ad as fa
 
