@@ -2,9 +2,8 @@
 
 No hipify, no torch JIT cache: every ``csrc/*.hip`` kernel file and ``csrc/*.cpp`` host file is
 compiled explicitly with ``hipcc --offload-arch=gfx950`` into ``build/obj`` and linked into an
-extension module that lives next to this file, so the built ``.so`` travels with the repository
-snapshot to the GPU box.  Objects are rebuilt only when a source or header is newer or the command that
-compiles them is another.
+extension module that lives next to this file, so the built ``.so`` travels with the tree.  Objects
+are rebuilt only when a source or header is newer or the command that compiles them is another.
 
 Usage:  python -m pytorch_cifar_amd._build [--force] [-v]
 """
